@@ -225,6 +225,44 @@ int mb_decode_step_meta(int batch, int max_pages, int page_size, const int32_t* 
                         int32_t* q_pos, int32_t* kv_len, int32_t* slot, mb_stream_t stream);
 
 /* ---------------------------------------------------------------------
+ * A ragged step's metadata on the device (K14): row b appends lengths[b]
+ * tokens (0 and more), the new tokens of all rows packed one row after the
+ * other. Replaces the host-side position and slot bookkeeping of
+ * FlexDecodeSession.forward (models/backbone/flex_decode.py:180-196) for
+ * chunks of any lengths. From kv_len [batch] (tokens cached before) and the
+ * page ids free_pages [n_free], handed out row by row in their order:
+ *   cu_q [batch + 1]      offsets of the rows in the packed stream
+ *   cu_pages [batch + 1]  pages opened by the rows before each (the last
+ *                         entry: all pages taken from free_pages)
+ *   new_len [batch]       kv_len + lengths (not kv_len's own memory)
+ *   block_table [batch, max_pages]  the opened pages' entries are written
+ *   q_pos, slot [tokens]  position and cache slot of every packed token;
+ *                         entries behind the last row's tokens get 0 and -1
+ * Negative lengths count as 0. A step that needs more pages than n_free or
+ * max_pages hold (status 3) or more than `tokens` tokens (status 7) writes
+ * what fits: tokens without a page get slot -1. All int32, device memory.
+ * ------------------------------------------------------------------- */
+int mb_chunk_meta(const int32_t* lengths, const int32_t* kv_len, int batch, int32_t* block_table, int max_pages,
+                  int page_size, const int32_t* free_pages, int n_free, int tokens, int32_t* cu_q,
+                  int32_t* cu_pages, int32_t* new_len, int32_t* q_pos, int32_t* slot, mb_stream_t stream);
+
+/* ---------------------------------------------------------------------
+ * Attention of ragged chunks over the paged cache (K15). Replaces
+ * models/backbone/flex_decode.py:226-229 for a step whose rows append
+ * different numbers of tokens: q [tokens, q_heads, head_dim] is packed (token
+ * t at q + t * q_stride elements), row b's tokens are cu_q[b] .. cu_q[b + 1] - 1
+ * and are the last of its kv_len[b] cached ones, so that the token at position
+ * p sees the row's slots 0..p (a token with p < 0 gets 0). out
+ * [tokens, q_heads, head_dim]; entries behind cu_q[batch] are left as they
+ * were. head_dim 64 or 128; page_size a multiple of 64; q, out and the pools
+ * 16-byte aligned, q_stride a multiple of 8.
+ * ------------------------------------------------------------------- */
+int mb_chunk_attention(const void* q, long long q_stride, const void* k_pool, const void* v_pool, int num_pages,
+                       const int32_t* block_table, int max_pages, const int32_t* cu_q, const int32_t* kv_len,
+                       int batch, int tokens, int q_heads, int kv_heads, int head_dim, int page_size, float scale,
+                       void* out, mb_stream_t stream);
+
+/* ---------------------------------------------------------------------
  * Decoder-layer glue.
  * mb_rmsnorm: sum_out = x + residual (bf16), norm_out = RMSNorm(sum) * w;
  *   with residual == NULL it normalises x (sum_out unused). Replaces the

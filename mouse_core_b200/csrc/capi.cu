@@ -410,6 +410,78 @@ int mb_decode_step_meta(int batch, int max_pages, int page_size, const int32_t* 
   return e == cudaSuccess ? MB_OK : cuda_fail(e, "decode step meta launch");
 }
 
+int mb_chunk_meta(const int32_t* lengths, const int32_t* kv_len, int batch, int32_t* block_table, int max_pages,
+                  int page_size, const int32_t* free_pages, int n_free, int tokens, int32_t* cu_q,
+                  int32_t* cu_pages, int32_t* new_len, int32_t* q_pos, int32_t* slot, mb_stream_t stream) {
+  if (batch < 0 || max_pages < 0 || n_free < 0 || tokens < 0 || page_size <= 0)
+    return fail(MB_ERR_INVALID_ARG, "batch, max_pages, n_free and tokens must be >= 0 and page_size > 0");
+  if (!cu_q || !cu_pages) return fail(MB_ERR_INVALID_ARG, "a required pointer is NULL");
+  if (batch > 0 && (!lengths || !kv_len || !new_len || (max_pages > 0 && !block_table)))
+    return fail(MB_ERR_INVALID_ARG, "a required pointer is NULL");
+  if ((tokens > 0 && (!q_pos || !slot)) || (n_free > 0 && !free_pages))
+    return fail(MB_ERR_INVALID_ARG, "a required pointer is NULL");
+  if (batch > 0 && (new_len == kv_len || new_len == lengths))
+    return fail(MB_ERR_INVALID_ARG, "new_len must not be kv_len's or lengths' memory");
+  mb::ChunkMetaParams p{};
+  p.lengths = lengths;
+  p.kv_len = kv_len;
+  p.block_table = block_table;
+  p.free_pages = free_pages;
+  p.batch = batch;
+  p.max_pages = max_pages;
+  p.page_size = page_size;
+  p.n_free = n_free;
+  p.tokens = tokens;
+  p.cu_q = cu_q;
+  p.cu_pages = cu_pages;
+  p.new_len = new_len;
+  p.q_pos = q_pos;
+  p.slot = slot;
+  cudaError_t e = mb::launch_chunk_meta(p, (cudaStream_t)stream);
+  return e == cudaSuccess ? MB_OK : cuda_fail(e, "chunk meta launch");
+}
+
+int mb_chunk_attention(const void* q, long long q_stride, const void* k_pool, const void* v_pool, int num_pages,
+                       const int32_t* block_table, int max_pages, const int32_t* cu_q, const int32_t* kv_len,
+                       int batch, int tokens, int q_heads, int kv_heads, int head_dim, int page_size, float scale,
+                       void* out, mb_stream_t stream) {
+  int rc = check_decode_shape(batch, tokens, q_heads, kv_heads, head_dim, page_size);
+  if (rc) return rc;
+  if (batch == 0 || tokens == 0) return MB_OK;
+  if (!q || !k_pool || !v_pool || !block_table || !cu_q || !kv_len || !out)
+    return fail(MB_ERR_INVALID_ARG, "a required pointer is NULL");
+  if (num_pages <= 0 || max_pages <= 0) return fail(MB_ERR_INVALID_ARG, "num_pages and max_pages must be > 0");
+  if (!aligned(k_pool, 16) || !aligned(v_pool, 16) || !aligned(q, 16) || !aligned(out, 16))
+    return fail(MB_ERR_INVALID_ARG, "q, out and the pools must be 16-byte aligned");
+  if (q_stride < (long long)q_heads * head_dim || q_stride % 8)
+    return fail(MB_ERR_INVALID_ARG, "q_stride must be a multiple of 8, at least q_heads * head_dim");
+  if ((long long)num_pages * kv_heads * page_size >= (1ll << 31))
+    return fail(MB_ERR_UNSUPPORTED, "pool too large for one layer (>= 2^31 rows)");
+  if ((long long)max_pages * page_size >= (1ll << 31))
+    return fail(MB_ERR_UNSUPPORTED, "a block table row must hold fewer than 2^31 tokens");
+  mb::ChunkParams p{};
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q_stride = q_stride;
+  p.k_pool = static_cast<const __nv_bfloat16*>(k_pool);
+  p.v_pool = static_cast<const __nv_bfloat16*>(v_pool);
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.block_table = block_table;
+  p.cu_q = cu_q;
+  p.kv_len = kv_len;
+  p.batch = batch;
+  p.tokens = tokens;
+  p.Hq = q_heads;
+  p.Hkv = kv_heads;
+  p.G = q_heads / kv_heads;
+  p.head_dim = head_dim;
+  p.max_pages = max_pages;
+  p.page_size = page_size;
+  p.num_pages = num_pages;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  cudaError_t e = mb::launch_chunk_attention(p, (cudaStream_t)stream);
+  return e == cudaSuccess ? MB_OK : cuda_fail(e, "chunk attention launch");
+}
+
 int mb_rmsnorm(const void* x, const void* residual, const void* weight, float eps, int rows, int dim, void* sum_out,
                void* norm_out, mb_stream_t stream) {
   if (rows < 0 || dim <= 0 || dim % 2) return fail(MB_ERR_INVALID_ARG, "rows >= 0 and an even dim > 0 required");

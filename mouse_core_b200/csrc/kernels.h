@@ -200,6 +200,37 @@ cudaError_t launch_decode_step_meta(int B, int width, int page_size, const int32
 cudaError_t launch_segment_meta(const int64_t* seq, int L, int tile, int64_t* pos_out, int32_t* run_start,
                                 int32_t* run_end, int32_t* tile_lo, int32_t* flags, cudaStream_t stream);
 
+// Ragged steps (chunk_meta.cu, chunk_attention.cu): row b appends
+// cu_q[b + 1] - cu_q[b] tokens, packed one row after the other.
+struct ChunkMetaParams {
+  const int32_t* lengths;     // [batch] new tokens
+  const int32_t* kv_len;      // [batch] cached tokens before the step
+  int32_t* block_table;       // [batch, max_pages]: the opened pages' entries are written
+  const int32_t* free_pages;  // [n_free] page ids in the order they are handed out
+  int batch, max_pages, page_size, n_free, tokens;
+  int32_t* cu_q;              // [batch + 1]
+  int32_t* cu_pages;          // [batch + 1]
+  int32_t* new_len;           // [batch]
+  int32_t* q_pos;             // [tokens]
+  int32_t* slot;              // [tokens]
+};
+cudaError_t launch_chunk_meta(const ChunkMetaParams& p, cudaStream_t stream);
+
+struct ChunkParams {
+  const __nv_bfloat16* q;       // [tokens, Hq, HD], tokens q_stride elements apart
+  const __nv_bfloat16* k_pool;  // [num_pages, Hkv, page, HD]
+  const __nv_bfloat16* v_pool;
+  __nv_bfloat16* out;           // [tokens, Hq, HD]
+  const int32_t* block_table;   // [batch, max_pages]
+  const int32_t* cu_q;          // [batch + 1]
+  const int32_t* kv_len;        // [batch] cached tokens, the new ones included
+  int batch, tokens, Hq, Hkv, G, head_dim;
+  int max_pages, page_size, num_pages;
+  long long q_stride;
+  float scale_log2;
+};
+cudaError_t launch_chunk_attention(const ChunkParams& p, cudaStream_t stream);
+
 // Token embedding (embed.cu).
 struct EmbedParams {
   const int32_t* types;        // [L] token type (modality) id

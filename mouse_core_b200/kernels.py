@@ -252,6 +252,92 @@ def decode_step_meta_launch(args: tuple, use_new_page: bool, stream: int) -> Non
     _count()
 
 
+def _same_device(ref: torch.Tensor, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != ref.device:
+            raise ValueError(f"{name} must be on {ref.device}, got {t.device}")
+
+
+def chunk_meta(lengths: torch.Tensor, kv_len: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
+               page_size: int, n_tokens: int):
+    """K14: the metadata of a ragged step in which row ``b`` appends
+    ``lengths[b]`` tokens (zero included) to its ``kv_len[b]`` cached ones, the
+    new tokens of all rows packed one row after the other.
+
+    All tensors are int32 on one device: ``lengths``, ``kv_len`` ``[B]``,
+    ``block_table`` ``[B, max_pages]`` (the entries of the pages that the step
+    opens are written in place) and ``free_pages``, the free pages' ids, handed
+    out row by row in their order. ``n_tokens`` is the packed stream's length
+    on the host, at least the sum of ``lengths``.
+
+    Returns ``(cu_q [B + 1], q_pos [n_tokens], slot [n_tokens], new_len [B],
+    cu_pages [B + 1])``: the rows' offsets in the stream, every token's
+    position and cache slot (0 and -1 behind the last row's tokens), the new
+    lengths, and the pages opened before each row (``cu_pages[B]``: pages taken
+    from ``free_pages``). A step that does not fit is reported through
+    ``_lib.device_status`` (3: out of pages or table columns, 7: out of
+    tokens) and its tokens without a page get slot -1."""
+    for name, t in (("lengths", lengths), ("kv_len", kv_len), ("block_table", block_table),
+                    ("free_pages", free_pages)):
+        _need(t, name, torch.int32)
+    B, T = lengths.numel(), int(n_tokens)
+    if lengths.ndim != 1 or kv_len.shape != lengths.shape or block_table.ndim != 2 or block_table.shape[0] != B:
+        raise ValueError("lengths and kv_len must be [B] and block_table [B, max_pages]")
+    if T < 0 or page_size <= 0:
+        raise ValueError("n_tokens must be >= 0 and page_size > 0")
+    _same_device(lengths, kv_len=kv_len, block_table=block_table, free_pages=free_pages)
+    with torch.cuda.device(lengths.device):
+        buf = torch.empty(3 * B + 2 + 2 * T, dtype=torch.int32, device=lengths.device)
+        cu_q, cu_pages, new_len, q_pos, slot = buf.split((B + 1, B + 1, B, T, T))
+        _lib.call("mb_chunk_meta", _p(lengths), _p(kv_len), B, _p(block_table), block_table.shape[1], int(page_size),
+                  _p(free_pages), free_pages.numel(), T, _p(cu_q), _p(cu_pages), _p(new_len), _p(q_pos), _p(slot),
+                  _stream(lengths))
+    _count()
+    return cu_q, q_pos, slot, new_len, cu_pages
+
+
+def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
+                    cu_q: torch.Tensor, kv_len: torch.Tensor, scale: float,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """K15: paged GQA attention of ragged chunks. q ``[T, Hq, hd]`` bf16 is the
+    packed stream (heads contiguous; tokens may be strided, e.g. a slice of a
+    fused projection): row ``b`` holds tokens ``cu_q[b] .. cu_q[b + 1] - 1``,
+    the last of its ``kv_len[b]`` cached ones, and the token at position ``p``
+    sees the row's cached slots ``0..p``. Pools ``[P, Hkv, page, hd]`` bf16 (one
+    layer, the new tokens' K/V already appended); block_table ``[B, max_pages]``,
+    cu_q ``[B + 1]``, kv_len ``[B]`` int32. Returns ``out [T, Hq, hd]``; tokens
+    behind ``cu_q[B]`` are left as they were."""
+    _need(q, "q", BF16, contiguous=False)
+    _need(k_pool, "k_pool", BF16)
+    _need(v_pool, "v_pool", BF16)
+    for name, t in (("block_table", block_table), ("cu_q", cu_q), ("kv_len", kv_len)):
+        _need(t, name, torch.int32)
+    if q.ndim != 3 or k_pool.ndim != 4 or k_pool.shape != v_pool.shape:
+        raise ValueError("q must be [T, Hq, hd] and the pools [P, Hkv, page, hd] of equal shape")
+    T, Hq, hd = q.shape
+    P, Hkv, page, hd2 = k_pool.shape
+    if hd2 != hd:
+        raise ValueError(f"head_dim mismatch: q {hd}, pool {hd2}")
+    if q.stride(2) != 1 or (Hq > 1 and q.stride(1) != hd):
+        raise ValueError("q's heads must be contiguous")
+    B = kv_len.numel()
+    if kv_len.ndim != 1 or cu_q.shape != (B + 1,) or block_table.ndim != 2 or block_table.shape[0] != B:
+        raise ValueError("block_table [B, max_pages], cu_q [B + 1] and kv_len [B] must match")
+    if out is not None:
+        _need(out, "out", BF16)
+        if out.shape != q.shape:
+            raise ValueError("out must have q's shape")
+    _same_device(q, k_pool=k_pool, v_pool=v_pool, block_table=block_table, cu_q=cu_q, kv_len=kv_len, out=out)
+    with torch.cuda.device(q.device):
+        if out is None:
+            out = torch.empty(T, Hq, hd, dtype=BF16, device=q.device)
+        _lib.call("mb_chunk_attention", _p(q), q.stride(0) if T > 1 else Hq * hd, _p(k_pool), _p(v_pool), P,
+                  _p(block_table), block_table.shape[1], _p(cu_q), _p(kv_len), B, T, Hq, Hkv, hd, page, float(scale),
+                  _p(out), _stream(q))
+    _count()
+    return out
+
+
 def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torch.Tensor | None = None):
     """Returns ``(sum, norm)``: ``sum = x + residual`` (or ``x``), ``norm = RMSNorm(sum) * weight``."""
     _need(x, "x", BF16)

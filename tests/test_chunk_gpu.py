@@ -1,0 +1,401 @@
+"""GPU parity of the ragged step: K14 (slot maps and block tables) against a
+loop over the rows, exactly, and K15 (attention of packed chunks over the paged
+cache) against its formula in 64 bits.
+
+Tolerance of K15, element by element. With p the softmax weights, o = sum p v
+and A = sum p |v| over the visible keys (64 bits): the kernel rounds the weights
+to bf16 before the second product (at most 2^-8 of each term: 2^-8 A), and the
+output to bf16 (2^-8 |o|); scores, exponentials, sums and the merge of split
+keys are held in fp32 (relative 2^-20 of a term or better). A quarter of a
+2^-8 of both is left for those: |out - o| <= (2^-8 + 2^-10) (A + |o|), plus
+the smallest bf16 step near zero."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+TOL = 2.0 ** -8 + 2.0 ** -10
+
+
+def _dev():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    from mouse_core_b200 import build
+
+    build.build()
+    return torch.device("cuda")
+
+
+def _status():
+    from mouse_core_b200 import _lib
+
+    return _lib.device_status()
+
+
+# ------------------------------------------------------------------ K14
+def _meta_reference(n, c, table, free, page, tokens):
+    """Loop over rows and tokens; a step that does not fit keeps what does."""
+    table = table.copy()
+    cu_q, cu_pages, pos, slot = [0], [0], np.zeros(tokens, np.int64), np.full(tokens, -1, np.int64)
+    t = taken = 0
+    for b in range(len(n)):
+        held, total = -(-c[b] // page), -(-(c[b] + n[b]) // page)
+        for col in range(held, total):
+            if taken < len(free) and col < table.shape[1]:
+                table[b, col] = free[taken]
+            taken += 1
+        for i in range(n[b]):
+            p = c[b] + i
+            if t < tokens:
+                pos[t] = p
+                col = p // page
+                fits = col < table.shape[1] and (col < held or cu_pages[-1] + col - held < len(free))
+                if fits and table[b, col] >= 0:
+                    slot[t] = table[b, col] * page + p % page
+            t += 1
+        cu_q.append(t)
+        cu_pages.append(taken)
+    return np.array(cu_q), pos, slot, np.array(n) + np.array(c), np.array(cu_pages), table
+
+
+def _meta_case(n, c, page, seed, extra_width=1, spare=3):
+    rng = np.random.default_rng(seed)
+    held = [-(-x // page) for x in c]
+    total = [-(-(x + y) // page) for x, y in zip(c, n)]
+    need = sum(t - h for t, h in zip(total, held))
+    width = max(total + [1]) + extra_width
+    ids = rng.permutation(sum(held) + need + spare).astype(np.int32)
+    table = np.full((len(n), width), -1, np.int32)
+    at = 0
+    for b, h in enumerate(held):
+        table[b, :h] = ids[at:at + h]
+        at += h
+    return table, ids[at:at + need + spare]
+
+
+def _check_meta(n, c, page, table, free, tokens, status=0):
+    dev = _dev()
+    from mouse_core_b200 import kernels as K
+
+    t = torch.from_numpy(table.copy()).to(dev)
+    got = K.chunk_meta(torch.tensor(n, dtype=torch.int32, device=dev), torch.tensor(c, dtype=torch.int32, device=dev), t,
+                       torch.from_numpy(free.copy()).to(dev), page, tokens)
+    assert _status() == status
+    ref = _meta_reference(n, c, table, free, page, tokens)
+    for name, g, r in zip(("cu_q", "q_pos", "slot", "new_len", "cu_pages", "block_table"), (*got, t), ref):
+        assert np.array_equal(g.cpu().numpy(), r), name
+
+
+@pytest.mark.parametrize("page", [1, 64, 128, 192])
+@pytest.mark.parametrize("rows,most,seed", [(1, 1, 0), (1, 700, 1), (5, 3, 2), (33, 200, 3), (1023, 4, 4), (1024, 4, 5),
+                                            (1025, 9, 6), (4100, 2, 7)])
+def test_chunk_meta_matches_the_row_loop(page, rows, most, seed):
+    rng = np.random.default_rng(seed)
+    n = rng.integers(0, most + 1, rows).tolist()
+    c = rng.integers(0, 5 * page, rows).tolist()
+    n[rng.integers(rows)] = most
+    c[0] = 0
+    if rows > 3:
+        c[1], n[2], c[3] = page, 0, 2 * page - 1  # a full page, a row that sits out, one slot left
+        n[0] = n[3] = 1
+    table, free = _meta_case(n, c, page, seed)
+    _check_meta(n, c, page, table, free, sum(n) + (seed % 3) * 7)
+
+
+def test_chunk_meta_edges():
+    _check_meta([], [], 64, np.zeros((0, 3), np.int32), np.zeros(0, np.int32), 0)
+    _check_meta([], [], 64, np.zeros((0, 3), np.int32), np.zeros(0, np.int32), 5)
+    _check_meta([0, 0], [0, 70], 64, *_meta_case([0, 0], [0, 70], 64, 1), 0)
+    n, c = [100000, 0, 1, 3], [17, 5, 64, 200000]
+    _check_meta(n, c, 64, *_meta_case(n, c, 64, 2), sum(n))
+
+
+def test_chunk_meta_reports_a_step_that_does_not_fit():
+    n, c = [70, 1, 130], [60, 64, 0]
+    table, free = _meta_case(n, c, 64, 3, spare=0)
+    _check_meta(n, c, 64, table, free[:3], sum(n), status=3)  # out of free pages
+    _check_meta(n, c, 64, np.ascontiguousarray(table[:, :2]), free, sum(n), status=3)  # out of table columns
+    _check_meta(n, c, 64, table, free, 150, status=7)  # out of tokens
+    _check_meta(n, c, 64, table, free, 0, status=7)
+
+
+def test_chunk_meta_refuses_bad_arguments():
+    dev = _dev()
+    from mouse_core_b200 import kernels as K
+
+    i = torch.zeros(2, dtype=torch.int32, device=dev)
+    table = torch.zeros(2, 4, dtype=torch.int32, device=dev)
+    for bad in ((i.long(), i, table, i, 64, 5), (i, i[:1], table, i, 64, 5), (i, i, table[:1], i, 64, 5),
+                (i, i, table.t(), i, 64, 5), (i, i, table, i, 64, -1), (i, i, table, i, 0, 5)):
+        with pytest.raises((TypeError, ValueError)):
+            K.chunk_meta(*bad)
+
+
+# ------------------------------------------------------------------ K15
+def _paged(rows, Hq, Hkv, hd, page, seed, poison=float("nan"), spread=1.0):
+    """Packed queries and a shuffled page pool for ``rows`` of (cached, new)
+    tokens. Every slot without a token holds ``poison`` and every table entry
+    without a page an id far outside the pool."""
+    g = torch.Generator("cuda").manual_seed(seed)
+    lens = [c + n for c, n in rows]
+    pages = [-(-x // page) for x in lens]
+    P = sum(pages) + 3
+    perm = torch.randperm(P, generator=g, device="cuda").tolist()
+    table = torch.full((len(rows), max(pages + [1]) + 1), 1 << 30, dtype=torch.int32)
+    kp = torch.full((P, Hkv, page, hd), poison, dtype=torch.bfloat16, device="cuda")
+    vp = kp.clone()
+    at = 0
+    for b, x in enumerate(lens):
+        for i in range(pages[b]):
+            table[b, i] = perm[at]
+            m = min(page, x - i * page)
+            kp[perm[at], :, :m] = (torch.randn(Hkv, m, hd, generator=g, device="cuda") * spread).bfloat16()
+            vp[perm[at], :, :m] = torch.randn(Hkv, m, hd, generator=g, device="cuda").bfloat16()
+            at += 1
+    T = sum(n for _, n in rows)
+    q = (torch.randn(T, Hq, hd, generator=g, device="cuda") * spread).bfloat16()
+    cu = torch.tensor(np.concatenate([[0], np.cumsum([n for _, n in rows])]), dtype=torch.int32, device="cuda")
+    return q, kp, vp, table.cuda(), cu, torch.tensor(lens, dtype=torch.int32, device="cuda")
+
+
+def _attention_reference(q, kp, vp, table, cu, kv_len, scale):
+    """(o, A) of the module's docstring in 64 bits, row by row."""
+    T, Hq, hd = q.shape
+    Hkv, page = kp.shape[1:3]
+    o = torch.zeros(T, Hq, hd, dtype=torch.float64, device=q.device)
+    A = torch.zeros_like(o)
+    cu = cu.tolist()
+    for b, length in enumerate(kv_len.tolist()):
+        n = cu[b + 1] - cu[b]
+        if n == 0 or length <= 0:
+            continue
+        ids = table[b, : -(-length // page)].long()
+        k = kp[ids].transpose(0, 1).flatten(1, 2)[:, :length].double()
+        v = vp[ids].transpose(0, 1).flatten(1, 2)[:, :length].double()
+        for lo in range(cu[b], cu[b + 1], 64):
+            hi = min(lo + 64, cu[b + 1])
+            s = torch.einsum("thgd,hkd->thgk", q[lo:hi].double().unflatten(1, (Hkv, -1)), k) * scale
+            pos = torch.arange(lo, hi, device=q.device) - cu[b] + length - n
+            seen = torch.arange(length, device=q.device) <= pos[:, None]
+            s.masked_fill_(~seen[:, None, None], -torch.inf)
+            w = torch.softmax(s, -1).nan_to_num(0.0)  # a token that sees nothing
+            o[lo:hi] = torch.einsum("thgk,hkd->thgd", w, v).flatten(1, 2)
+            A[lo:hi] = torch.einsum("thgk,hkd->thgd", w, v.abs()).flatten(1, 2)
+    return o, A
+
+
+def _check(out, ref, what=""):
+    o, A = ref
+    err = (out.double() - o).abs()
+    assert bool(torch.isfinite(out.float()).all()), f"{what}: not finite"
+    over = (err / (TOL * (A + o.abs()) + 1e-30)).max().item() if out.numel() else 0.0
+    assert over <= 1.0, f"{what}: error {over:.2f} times the bound"
+
+
+CASES = {
+    # name: (rows of (cached, new), Hq, Hkv, hd, page)
+    "one_token": ([(0, 1)], 16, 8, 128, 128),
+    "one_token_cached": ([(300, 1)], 16, 8, 128, 128),
+    "step_with_idle_rows": ([(64, 1), (0, 0), (127, 1), (128, 1), (700, 0), (2049, 1), (5, 1)], 16, 8, 128, 128),
+    "transitions_hd64": ([(9000, 4), (63, 3), (64, 0), (1, 2), (4095, 1), (130, 4)], 32, 8, 64, 64),
+    "at_most_16_query_rows": ([(500, 8), (31, 7), (128, 5)], 4, 2, 128, 64),
+    "just_over_16_query_rows": ([(500, 9), (31, 17), (128, 1)], 4, 2, 128, 64),
+    "windows_from_empty": ([(0, 1024), (0, 1), (0, 129), (0, 64), (0, 65), (0, 257)], 16, 8, 128, 128),
+    "windows_hd64": ([(0, 500), (0, 33), (0, 1000), (0, 31), (0, 32)], 32, 8, 64, 64),
+    "mixed": ([(1500, 1), (0, 300), (10, 0), (777, 1), (200, 130), (4000, 1), (3, 2)], 16, 8, 128, 128),
+    "chunk_over_prefix": ([(1023, 256), (1024, 256), (2500, 255), (40, 256)], 16, 8, 128, 128),
+    "no_gqa": ([(100, 300), (513, 1), (0, 256), (5, 257)], 4, 4, 128, 128),
+    "group_of_3": ([(100, 50), (1000, 1), (0, 43), (64, 84), (63, 85), (7, 6)], 12, 4, 128, 64),
+    "group_of_7": ([(100, 50), (1000, 1), (0, 18), (64, 36), (63, 37), (7, 2), (700, 3)], 14, 2, 64, 128),
+    "group_of_16": ([(100, 50), (1000, 1), (0, 8), (64, 16), (63, 17), (7, 2)], 16, 1, 128, 192),
+    "group_of_32": ([(100, 9), (1000, 1), (0, 4), (64, 8)], 32, 1, 64, 64),
+    "one_head": ([(0, 5), (600, 1), (128, 128), (127, 257)], 1, 1, 64, 64),
+    "long_axis_few_rows": ([(40000, 1), (30001, 3)], 16, 8, 128, 128),
+    "long_axis_chunk": ([(20011, 200)], 16, 8, 128, 128),
+    "long_axis_hd64": ([(33333, 5), (65000, 1)], 32, 8, 64, 64),
+    "many_rows": ([(17 * i % 900, (i * 7) % 3) for i in range(1500)], 4, 2, 64, 64),
+    "large_pages": ([(1000, 3), (0, 700), (319, 2)], 8, 2, 128, 320),
+}
+
+
+@pytest.mark.parametrize("name", list(CASES))
+def test_chunk_attention_matches_the_formula(name):
+    _dev()
+    from mouse_core_b200 import kernels as K
+
+    rows, Hq, Hkv, hd, page = CASES[name]
+    args = _paged(rows, Hq, Hkv, hd, page, seed=len(name))
+    out = K.chunk_attention(*args, hd ** -0.5)
+    assert _status() == 0
+    _check(out, _attention_reference(*args, hd ** -0.5), name)
+    again = K.chunk_attention(*args, hd ** -0.5)
+    assert torch.equal(out, again), "the same call twice gives other bits"
+
+
+@pytest.mark.parametrize("poison", [float("inf"), float("-inf"), torch.finfo(torch.bfloat16).min])
+def test_slots_without_a_token_are_not_read(poison):
+    _dev()
+    from mouse_core_b200 import kernels as K
+
+    rows = [(1, 1), (63, 1), (64, 2), (100, 40), (0, 129), (191, 1)]
+    args = _paged(rows, 16, 8, 128, 64, seed=5, poison=poison)
+    out = K.chunk_attention(*args, 128 ** -0.5)
+    assert _status() == 0
+    _check(out, _attention_reference(*args, 128 ** -0.5))
+
+
+def test_large_scores():
+    """Scores in the hundreds: one key carries nearly all the weight."""
+    _dev()
+    from mouse_core_b200 import kernels as K
+
+    rows = [(900, 1), (300, 200), (0, 70), (2300, 3)]
+    for hd in (64, 128):
+        args = _paged(rows, 8, 4, hd, 64, seed=9, spread=4.0)
+        out = K.chunk_attention(*args, hd ** -0.5)
+        assert _status() == 0
+        _check(out, _attention_reference(*args, hd ** -0.5))
+
+
+def test_tokens_before_the_cache_get_zero():
+    """kv_len below the row's token count: the first tokens sit at negative positions."""
+    _dev()
+    from mouse_core_b200 import kernels as K
+
+    q, kp, vp, table, cu, kv_len = _paged([(0, 5), (0, 200), (0, 1), (0, 40)], 16, 8, 128, 128, seed=3)
+    kv_len = torch.tensor([3, 70, 0, 0], dtype=torch.int32, device="cuda")
+    out = K.chunk_attention(q, kp, vp, table, cu, kv_len, 0.1)
+    assert _status() == 0
+    assert bool((out[:2] == 0).all()) and bool((out[5:135] == 0).all()) and bool((out[205:] == 0).all())
+    _check(out, _attention_reference(q, kp, vp, table, cu, kv_len, 0.1))
+
+
+def test_strided_queries_and_rows_behind_the_last_sequence():
+    _dev()
+    from mouse_core_b200 import kernels as K
+
+    rows, Hq, Hkv, hd = [(100, 1), (30, 70), (260, 2)], 16, 8, 128
+    q, kp, vp, table, cu, kv_len = _paged(rows, Hq, Hkv, hd, 64, seed=11)
+    ref = _attention_reference(q, kp, vp, table, cu, kv_len, 0.1)
+    T, extra = q.shape[0], 37
+    fused = torch.full((T + extra, (Hq + 2 * Hkv) * hd), float("nan"), dtype=torch.bfloat16, device="cuda")
+    view = fused[:, : Hq * hd].unflatten(1, (Hq, hd))
+    view[:T] = q
+    out = torch.full((T + extra, Hq, hd), 7.0, dtype=torch.bfloat16, device="cuda")
+    got = K.chunk_attention(view, kp, vp, table, cu, kv_len, 0.1, out=out)
+    assert got is out and _status() == 0
+    _check(out[:T], ref)
+    assert bool((out[T:] == 7.0).all())
+
+
+def test_empty_calls():
+    _dev()
+    from mouse_core_b200 import kernels as K
+
+    q, kp, vp, table, cu, kv_len = _paged([(10, 0), (0, 0)], 4, 2, 64, 64, seed=1)
+    assert K.chunk_attention(q, kp, vp, table, cu, kv_len, 0.1).shape == (0, 4, 64)
+    out = torch.full((3, 4, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    K.chunk_attention(torch.zeros_like(out), kp, vp, table, cu, kv_len, 0.1, out=out)  # no row has a token
+    assert _status() == 0 and bool((out == 7.0).all())
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    K.chunk_attention(torch.zeros_like(out), kp, vp, table[:0], cu[:1], none, 0.1, out=out)
+    assert _status() == 0 and bool((out == 7.0).all())
+
+
+def test_a_page_outside_the_pool_reads_as_zero_and_is_reported():
+    _dev()
+    from mouse_core_b200 import kernels as K
+
+    for rows in ([(500, 1), (40, 1)], [(400, 100), (40, 1)]):
+        q, kp, vp, table, cu, kv_len = _paged(rows, 16, 8, 128, 128, seed=2)
+        bad = table.clone()
+        bad[0, 1] = -1
+        kz, vz = kp.clone(), vp.clone()
+        kz[table[0, 1]] = vz[table[0, 1]] = 0
+        out = K.chunk_attention(q, kp, vp, bad, cu, kv_len, 0.1)
+        assert _status() == 3
+        _check(out, _attention_reference(q, kz, vz, table, cu, kv_len, 0.1))
+
+
+def test_a_pool_beyond_32_bit_offsets():
+    dev = _dev()
+    from mouse_core_b200 import kernels as K
+
+    Hkv, page, hd = 8, 128, 128
+    P = (1 << 31) // (Hkv * page * hd) + 40  # the last pages' elements lie past 2^31
+    kp, vp = (torch.zeros(P, Hkv, page, hd, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    g = torch.Generator("cuda").manual_seed(4)
+    rows = [(500, 1), (300, 140), (2600, 3)]
+    ids = torch.arange(P - 30, P, device=dev)
+    kp[ids] = torch.randn(30, Hkv, page, hd, generator=g, device=dev).bfloat16()
+    vp[ids] = torch.randn(30, Hkv, page, hd, generator=g, device=dev).bfloat16()
+    table = torch.full((3, 21), -1, dtype=torch.int32, device=dev)
+    table[0, :4], table[1, :4], table[2, :21] = ids[:4].int(), ids[4:8].int(), ids[9:].int()
+    q = torch.randn(144, 16, hd, generator=g, device=dev).bfloat16()
+    cu = torch.tensor([0, 1, 141, 144], dtype=torch.int32, device=dev)
+    kv_len = torch.tensor([c + n for c, n in rows], dtype=torch.int32, device=dev)
+    out = K.chunk_attention(q, kp, vp, table, cu, kv_len, 0.1)
+    assert _status() == 0
+    _check(out, _attention_reference(q, kp, vp, table, cu, kv_len, 0.1))
+
+
+def test_refusals_of_the_attention_wrapper():
+    _dev()
+    from mouse_core_b200 import kernels as K
+
+    q, kp, vp, table, cu, kv_len = _paged([(10, 3), (5, 1)], 4, 2, 64, 64, seed=1)
+    good = dict(q=q, k_pool=kp, v_pool=vp, block_table=table, cu_q=cu, kv_len=kv_len, scale=0.1)
+    bad = [dict(q=q.float()), dict(q=q[0]), dict(q=q.transpose(1, 2).contiguous().transpose(1, 2)),
+           dict(k_pool=kp.transpose(1, 2)), dict(v_pool=vp[:, :1].contiguous()), dict(q=q[:, :, :32].contiguous()),
+           dict(cu_q=cu[:2]), dict(cu_q=cu.long()), dict(kv_len=kv_len[:1]), dict(block_table=table[:1]),
+           dict(out=torch.empty(2, 4, 64, dtype=torch.bfloat16, device="cuda")), dict(out=torch.empty_like(q).float()),
+           dict(q=q[:, :3].contiguous()), dict(block_table=table.cpu())]
+    for b in bad:
+        with pytest.raises((TypeError, ValueError, RuntimeError)):
+            K.chunk_attention(**{**good, **b})
+    assert _status() == 0
+
+
+def test_other_streams_and_captured_graphs():
+    """Calls in flight together on two streams, and a captured call replayed
+    after its inputs changed, each on its own workspace."""
+    _dev()
+    from mouse_core_b200 import kernels as K
+
+    a = _paged([(3000, 1), (0, 200), (77, 3), (9000, 2)], 16, 8, 128, 128, seed=21)
+    b = _paged([(50, 130), (6000, 1), (1, 1)], 32, 8, 64, 64, seed=22)
+    ref_a, ref_b = _attention_reference(*a, 0.1), _attention_reference(*b, 0.1)
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    outs = []
+    for _ in range(20):
+        with torch.cuda.stream(s1):
+            outs.append((K.chunk_attention(*a, 0.1), ref_a))
+        with torch.cuda.stream(s2):
+            outs.append((K.chunk_attention(*b, 0.1), ref_b))
+    torch.cuda.synchronize()
+    assert _status() == 0
+    for out, ref in outs:
+        _check(out, ref)
+
+    q, kp, vp, table, cu, kv_len = (t.clone() for t in a)
+    K.chunk_attention(q, kp, vp, table, cu, kv_len, 0.1)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = K.chunk_attention(q, kp, vp, table, cu, kv_len, 0.1)
+    graph.replay()
+    torch.cuda.synchronize()
+    _check(out, ref_a)
+    # The same buffers with other lengths and another split of the tokens over the rows.
+    cu.copy_(torch.tensor([0, 150, 151, 151, 206], dtype=torch.int32))
+    kv_len.copy_(torch.tensor([2000, 199, 80, 9002], dtype=torch.int32))
+    q.copy_(q.flip(0))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert _status() == 0
+    _check(out, _attention_reference(q, kp, vp, table, cu, kv_len, 0.1))
