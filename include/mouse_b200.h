@@ -254,13 +254,29 @@ int mb_chunk_meta(const int32_t* lengths, const int32_t* kv_len, int batch, int3
  * and are the last of its kv_len[b] cached ones, so that the token at position
  * p sees the row's slots 0..p (a token with p < 0 gets 0). out
  * [tokens, q_heads, head_dim]; entries behind cu_q[batch] are left as they
- * were. head_dim 64 or 128; page_size a multiple of 64; q, out and the pools
- * 16-byte aligned, q_stride a multiple of 8.
+ * were. head_dim 64 or 128; at most 128 q-heads per kv-head; page_size a
+ * multiple of 64; q, out and the pools 16-byte aligned, q_stride a multiple
+ * of 8; scale > 0. Slots of a page behind the row's last token are not read
+ * as values (they may hold NaN). A page id outside the pool reads as zeros
+ * and sets status 3, as does a kv_len beyond max_pages * page_size (the keys
+ * past the table are left out); offsets that overlap set status 7 and write
+ * nothing.
+ *
+ * mb_chunk_plan builds the step's work list in `workspace` from cu_q and
+ * kv_len alone, so one plan serves every layer of a step: pass plan_ready = 1
+ * with the same sizes; 0 builds it in the call. Needs
+ * mb_chunk_workspace_bytes(...) bytes, 256-byte aligned, on the device that is
+ * current. Calls that may overlap on the GPU need workspaces of their own.
+ * The output does not depend on how the work was scheduled (bit for bit).
  * ------------------------------------------------------------------- */
+size_t mb_chunk_workspace_bytes(int batch, int tokens, int q_heads, int kv_heads, int head_dim);
+int mb_chunk_plan(const int32_t* cu_q, const int32_t* kv_len, int batch, int tokens, int q_heads, int kv_heads,
+                  int head_dim, int page_size, int max_pages, void* workspace, size_t workspace_bytes,
+                  mb_stream_t stream);
 int mb_chunk_attention(const void* q, long long q_stride, const void* k_pool, const void* v_pool, int num_pages,
                        const int32_t* block_table, int max_pages, const int32_t* cu_q, const int32_t* kv_len,
                        int batch, int tokens, int q_heads, int kv_heads, int head_dim, int page_size, float scale,
-                       void* out, mb_stream_t stream);
+                       int plan_ready, void* out, void* workspace, size_t workspace_bytes, mb_stream_t stream);
 
 /* ---------------------------------------------------------------------
  * Decoder-layer glue.

@@ -39,8 +39,10 @@ PROTOTYPES = {
     "mb_decode_step_meta": (_c_int, [_c_int, _c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _vp]),
     "mb_chunk_meta": (_c_int, [_vp, _vp, _c_int, _vp, _c_int, _c_int, _vp, _c_int, _c_int, _vp, _vp, _vp, _vp, _vp,
                                _vp]),
+    "mb_chunk_workspace_bytes": (_c_size, [_c_int] * 5),
+    "mb_chunk_plan": (_c_int, [_vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _c_size, _vp]),
     "mb_chunk_attention": (_c_int, [_vp, _c_ll, _vp, _vp, _c_int, _vp, _c_int, _vp, _vp, _c_int, _c_int, _c_int,
-                                    _c_int, _c_int, _c_int, _c_float, _vp, _vp]),
+                                    _c_int, _c_int, _c_int, _c_float, _c_int, _vp, _vp, _c_size, _vp]),
     "mb_rmsnorm": (_c_int, [_vp, _vp, _vp, _c_float, _c_int, _c_int, _vp, _vp, _vp]),
     "mb_embed_tokens": (_c_int, [_vp, _vp, _vp, _c_ll, _c_int, _vp, _vp, _vp, _c_int, _vp, _vp, _c_int,
                                  _c_float, _vp, _c_int, _vp]),

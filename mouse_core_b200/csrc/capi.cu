@@ -69,6 +69,24 @@ int encode_token_map(CUtensorMap* map, const void* base, int L, int heads, int h
   return MB_OK;
 }
 
+// 3-D view {head_dim, heads, tokens} of a packed stream whose tokens lie
+// `stride` elements apart: boxes of 64 elements x G heads x n tokens (a tile's
+// query rows, token by token), 128B swizzle.
+int encode_group_map(CUtensorMap* map, const void* base, int tokens, int heads, int head_dim, long long stride, int G,
+                     int n) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(MB_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)heads, (cuuint64_t)tokens};
+  cuuint64_t strides[2] = {(cuuint64_t)head_dim * 2, (cuuint64_t)stride * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)n};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MB_ERR_CUDA, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+  return MB_OK;
+}
+
 // A row-major bf16 matrix [rows, cols] read in boxes of 64 columns x 128
 // rows with the 128-byte swizzle (the K-major operand layout of tcgen05).
 int encode_matrix_map(CUtensorMap* map, const void* base, long long rows, int cols) {
@@ -441,44 +459,104 @@ int mb_chunk_meta(const int32_t* lengths, const int32_t* kv_len, int batch, int3
   return e == cudaSuccess ? MB_OK : cuda_fail(e, "chunk meta launch");
 }
 
-int mb_chunk_attention(const void* q, long long q_stride, const void* k_pool, const void* v_pool, int num_pages,
-                       const int32_t* block_table, int max_pages, const int32_t* cu_q, const int32_t* kv_len,
-                       int batch, int tokens, int q_heads, int kv_heads, int head_dim, int page_size, float scale,
-                       void* out, mb_stream_t stream) {
+size_t mb_chunk_workspace_bytes(int batch, int tokens, int q_heads, int kv_heads, int head_dim) {
+  if (batch <= 0 || tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || q_heads / kv_heads > 128)
+    return 0;
+  if (head_dim != 64 && head_dim != 128) return 0;
+  mb::ChunkLayout lay;
+  return mb::chunk_layout(batch, tokens, q_heads, kv_heads, head_dim, mb::num_sms(), &lay);
+}
+
+}  // extern "C"
+
+namespace {
+// The arguments that the plan and the attention share.
+int chunk_common(mb::ChunkParams* p, mb::ChunkLayout* lay, const int32_t* cu_q, const int32_t* kv_len, int batch,
+                 int tokens, int q_heads, int kv_heads, int head_dim, int page_size, int max_pages, void* workspace,
+                 size_t workspace_bytes) {
+  if (!cu_q || !kv_len) return fail(MB_ERR_INVALID_ARG, "a required pointer is NULL");
+  if (max_pages <= 0) return fail(MB_ERR_INVALID_ARG, "max_pages must be > 0");
+  if (q_heads / kv_heads > 128) return fail(MB_ERR_UNSUPPORTED, "at most 128 q-heads per kv-head");
+  if ((long long)max_pages * page_size >= (1ll << 31))
+    return fail(MB_ERR_UNSUPPORTED, "a block table row must hold fewer than 2^31 tokens");
+  const int sms = mb::num_sms();
+  const size_t need = mb::chunk_layout(batch, tokens, q_heads, kv_heads, head_dim, sms, lay);
+  if (lay->max_entries * kv_heads >= (1ull << 31)) return fail(MB_ERR_UNSUPPORTED, "too many tiles for one step");
+  if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
+    return fail(MB_ERR_WORKSPACE, "workspace needs " + std::to_string(need) + " bytes, 256-byte aligned");
+  p->cu_q = cu_q;
+  p->kv_len = kv_len;
+  p->batch = batch;
+  p->tokens = tokens;
+  p->Hq = q_heads;
+  p->Hkv = kv_heads;
+  p->G = q_heads / kv_heads;
+  p->head_dim = head_dim;
+  p->max_pages = max_pages;
+  p->page_size = page_size;
+  p->key_limit = max_pages * page_size;
+  p->sub_tokens = mb::chunk_sub_tokens(p->G);
+  p->small_rows = p->G <= 16 ? 16 / p->G * p->G : 0;
+  return MB_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int mb_chunk_plan(const int32_t* cu_q, const int32_t* kv_len, int batch, int tokens, int q_heads, int kv_heads,
+                  int head_dim, int page_size, int max_pages, void* workspace, size_t workspace_bytes,
+                  mb_stream_t stream) {
   int rc = check_decode_shape(batch, tokens, q_heads, kv_heads, head_dim, page_size);
   if (rc) return rc;
   if (batch == 0 || tokens == 0) return MB_OK;
-  if (!q || !k_pool || !v_pool || !block_table || !cu_q || !kv_len || !out)
-    return fail(MB_ERR_INVALID_ARG, "a required pointer is NULL");
-  if (num_pages <= 0 || max_pages <= 0) return fail(MB_ERR_INVALID_ARG, "num_pages and max_pages must be > 0");
+  mb::ChunkParams p{};
+  mb::ChunkLayout lay{};
+  rc = chunk_common(&p, &lay, cu_q, kv_len, batch, tokens, q_heads, kv_heads, head_dim, page_size, max_pages,
+                    workspace, workspace_bytes);
+  if (rc) return rc;
+  cudaError_t e =
+      mb::launch_chunk_plan(p, lay, static_cast<uint8_t*>(workspace), mb::num_sms(), (cudaStream_t)stream);
+  return e == cudaSuccess ? MB_OK : cuda_fail(e, "chunk plan launch");
+}
+
+int mb_chunk_attention(const void* q, long long q_stride, const void* k_pool, const void* v_pool, int num_pages,
+                       const int32_t* block_table, int max_pages, const int32_t* cu_q, const int32_t* kv_len,
+                       int batch, int tokens, int q_heads, int kv_heads, int head_dim, int page_size, float scale,
+                       int plan_ready, void* out, void* workspace, size_t workspace_bytes, mb_stream_t stream) {
+  int rc = check_decode_shape(batch, tokens, q_heads, kv_heads, head_dim, page_size);
+  if (rc) return rc;
+  if (batch == 0 || tokens == 0) return MB_OK;
+  if (!q || !k_pool || !v_pool || !block_table || !out) return fail(MB_ERR_INVALID_ARG, "a required pointer is NULL");
+  if (num_pages <= 0) return fail(MB_ERR_INVALID_ARG, "num_pages must be > 0");
   if (!aligned(k_pool, 16) || !aligned(v_pool, 16) || !aligned(q, 16) || !aligned(out, 16))
     return fail(MB_ERR_INVALID_ARG, "q, out and the pools must be 16-byte aligned");
-  if (q_stride < (long long)q_heads * head_dim || q_stride % 8)
+  if (q_stride < (long long)q_heads * head_dim || q_stride % 8 || q_stride >= (1ll << 38))
     return fail(MB_ERR_INVALID_ARG, "q_stride must be a multiple of 8, at least q_heads * head_dim");
-  if ((long long)num_pages * kv_heads * page_size >= (1ll << 31))
-    return fail(MB_ERR_UNSUPPORTED, "pool too large for one layer (>= 2^31 rows)");
-  if ((long long)max_pages * page_size >= (1ll << 31))
-    return fail(MB_ERR_UNSUPPORTED, "a block table row must hold fewer than 2^31 tokens");
+  if (!(scale >= 0x1p-40f && scale <= 0x1p40f)) return fail(MB_ERR_INVALID_ARG, "scale must be positive and finite");
+  const long long rows = (long long)num_pages * kv_heads * page_size;
+  if (rows >= (1ll << 31)) return fail(MB_ERR_UNSUPPORTED, "pool too large for one layer (>= 2^31 rows)");
   mb::ChunkParams p{};
-  p.q = static_cast<const __nv_bfloat16*>(q);
-  p.q_stride = q_stride;
-  p.k_pool = static_cast<const __nv_bfloat16*>(k_pool);
-  p.v_pool = static_cast<const __nv_bfloat16*>(v_pool);
-  p.out = static_cast<__nv_bfloat16*>(out);
+  mb::ChunkLayout lay{};
+  rc = chunk_common(&p, &lay, cu_q, kv_len, batch, tokens, q_heads, kv_heads, head_dim, page_size, max_pages,
+                    workspace, workspace_bytes);
+  if (rc) return rc;
   p.block_table = block_table;
-  p.cu_q = cu_q;
-  p.kv_len = kv_len;
-  p.batch = batch;
-  p.tokens = tokens;
-  p.Hq = q_heads;
-  p.Hkv = kv_heads;
-  p.G = q_heads / kv_heads;
-  p.head_dim = head_dim;
-  p.max_pages = max_pages;
-  p.page_size = page_size;
   p.num_pages = num_pages;
+  p.out = static_cast<__nv_bfloat16*>(out);
   p.scale_log2 = scale * 1.4426950408889634f;
-  cudaError_t e = mb::launch_chunk_attention(p, (cudaStream_t)stream);
+  CUtensorMap qm, sqm, km, vm;
+  if ((rc = encode_group_map(&qm, q, tokens, q_heads, head_dim, q_stride, p.G, p.sub_tokens))) return rc;
+  sqm = qm;
+  if (p.G <= 16 && (rc = encode_group_map(&sqm, q, tokens, q_heads, head_dim, q_stride, p.G, 16 / p.G))) return rc;
+  if ((rc = encode_pool_map(&km, k_pool, rows, head_dim))) return rc;
+  if ((rc = encode_pool_map(&vm, v_pool, rows, head_dim))) return rc;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const int sms = mb::num_sms();
+  if (!plan_ready) {
+    cudaError_t e = mb::launch_chunk_plan(p, lay, ws, sms, (cudaStream_t)stream);
+    if (e != cudaSuccess) return cuda_fail(e, "chunk plan launch");
+  }
+  cudaError_t e = mb::launch_chunk_attention(qm, sqm, km, vm, p, lay, ws, sms, (cudaStream_t)stream);
   return e == cudaSuccess ? MB_OK : cuda_fail(e, "chunk attention launch");
 }
 

@@ -152,6 +152,28 @@ __device__ __forceinline__ bool mbar_wait_abortable(uint64_t* bar, uint32_t pari
   }
 }
 
+// mbar_wait_abortable off the critical path: the warp sleeps between polls.
+__device__ __forceinline__ bool mbar_wait_sleepy_abortable(uint64_t* bar, uint32_t parity, int code, int* abort) {
+  volatile int* ab = abort;
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long limit = wait_limit();
+  const long long t0 = clock64();
+  while (true) {
+    if (*ab) return false;
+    if (clock64() - t0 > limit) {
+      report(code);
+      *ab = 1;
+      return false;
+    }
+    __nanosleep(128);
+    if (mbar_try_wait(bar, parity)) return true;
+  }
+}
+
+// This thread's shared-memory accesses so far come before the asynchronous
+// proxy's (TMA, tcgen05) that a later barrier orders behind them.
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
 // Wait for a phase that this CTA's own in-flight copies complete (a TMA load
 // it issued) before the CTA exits; bounded by kDrainCycles, not by the
 // host-set limit.

@@ -216,20 +216,40 @@ struct ChunkMetaParams {
 };
 cudaError_t launch_chunk_meta(const ChunkMetaParams& p, cudaStream_t stream);
 
+struct ChunkEntry;
 struct ChunkParams {
-  const __nv_bfloat16* q;       // [tokens, Hq, HD], tokens q_stride elements apart
-  const __nv_bfloat16* k_pool;  // [num_pages, Hkv, page, HD]
-  const __nv_bfloat16* v_pool;
-  __nv_bfloat16* out;           // [tokens, Hq, HD]
-  const int32_t* block_table;   // [batch, max_pages]
-  const int32_t* cu_q;          // [batch + 1]
-  const int32_t* kv_len;        // [batch] cached tokens, the new ones included
+  __nv_bfloat16* out;          // [tokens, Hq, HD]
+  const int32_t* block_table;  // [batch, max_pages]
+  const int32_t* cu_q;         // [batch + 1]
+  const int32_t* kv_len;       // [batch] cached tokens, the new ones included
   int batch, tokens, Hq, Hkv, G, head_dim;
   int max_pages, page_size, num_pages;
-  long long q_stride;
+  int key_limit;               // max_pages * page_size
+  int sub_tokens;              // tokens of a 128-query-row sub-tile
+  int small_rows;              // query rows that the small tiles' Q box holds (G <= 16)
   float scale_log2;
+  // the plan and the split tiles' partials (inside the caller's workspace)
+  const ChunkEntry* entries;
+  int* head;
+  int* counters;
+  float2* part_ml;
+  float* part_o;
+  int part_rows;
 };
-cudaError_t launch_chunk_attention(const ChunkParams& p, cudaStream_t stream);
+struct ChunkLayout {
+  size_t max_entries, max_slots;
+  int part_rows;
+  size_t head, entries, counters, part_ml, part_o, total;
+};
+int chunk_sub_tokens(int G);
+size_t chunk_layout(int batch, int tokens, int Hq, int Hkv, int head_dim, int sms, ChunkLayout* lay);
+cudaError_t launch_chunk_plan(const ChunkParams& p, const ChunkLayout& lay, uint8_t* ws, int sms,
+                              cudaStream_t stream);
+// qm / sqm: 3-D token maps with boxes of a sub-tile's / a small tile's queries;
+// km / vm: the decode kernel's 64 x 64-box maps of one layer's K / V pool.
+cudaError_t launch_chunk_attention(const CUtensorMap& qm, const CUtensorMap& sqm, const CUtensorMap& km,
+                                   const CUtensorMap& vm, ChunkParams p, const ChunkLayout& lay, uint8_t* ws, int sms,
+                                   cudaStream_t stream);
 
 // Token embedding (embed.cu).
 struct EmbedParams {

@@ -296,9 +296,30 @@ def chunk_meta(lengths: torch.Tensor, kv_len: torch.Tensor, block_table: torch.T
     return cu_q, q_pos, slot, new_len, cu_pages
 
 
+def chunk_workspace_bytes(batch: int, tokens: int, q_heads: int, kv_heads: int, head_dim: int) -> int:
+    """Workspace of ``chunk_plan`` and ``chunk_attention`` on the current device."""
+    return int(_lib.load().mb_chunk_workspace_bytes(batch, tokens, q_heads, kv_heads, head_dim))
+
+
+def chunk_plan(cu_q: torch.Tensor, kv_len: torch.Tensor, tokens: int, q_heads: int, kv_heads: int, head_dim: int,
+               page_size: int, max_pages: int, workspace: torch.Tensor) -> None:
+    """The work list of a ragged step, for ``chunk_attention(...,
+    plan_ready=True)`` with the same sizes in every layer of the step."""
+    for name, t in (("cu_q", cu_q), ("kv_len", kv_len)):
+        _need(t, name, torch.int32)
+    _need(workspace, "workspace", torch.uint8)
+    if kv_len.ndim != 1 or cu_q.shape != (kv_len.numel() + 1,):
+        raise ValueError("cu_q [B + 1] and kv_len [B] must match")
+    _same_device(cu_q, kv_len=kv_len, workspace=workspace)
+    with torch.cuda.device(cu_q.device):
+        _lib.call("mb_chunk_plan", _p(cu_q), _p(kv_len), kv_len.numel(), int(tokens), q_heads, kv_heads, head_dim,
+                  int(page_size), int(max_pages), _p(workspace), workspace.numel(), _stream(cu_q))
+    _count()
+
+
 def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
-                    cu_q: torch.Tensor, kv_len: torch.Tensor, scale: float,
-                    out: torch.Tensor | None = None) -> torch.Tensor:
+                    cu_q: torch.Tensor, kv_len: torch.Tensor, scale: float, out: torch.Tensor | None = None,
+                    workspace: torch.Tensor | None = None, plan_ready: bool = False) -> torch.Tensor:
     """K15: paged GQA attention of ragged chunks. q ``[T, Hq, hd]`` bf16 is the
     packed stream (heads contiguous; tokens may be strided, e.g. a slice of a
     fused projection): row ``b`` holds tokens ``cu_q[b] .. cu_q[b + 1] - 1``,
@@ -306,7 +327,9 @@ def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     sees the row's cached slots ``0..p``. Pools ``[P, Hkv, page, hd]`` bf16 (one
     layer, the new tokens' K/V already appended); block_table ``[B, max_pages]``,
     cu_q ``[B + 1]``, kv_len ``[B]`` int32. Returns ``out [T, Hq, hd]``; tokens
-    behind ``cu_q[B]`` are left as they were."""
+    behind ``cu_q[B]`` are left as they were. ``workspace`` (uint8, at least
+    ``chunk_workspace_bytes``) is allocated for the call when not given;
+    ``plan_ready`` takes the work list that ``chunk_plan`` left in it."""
     _need(q, "q", BF16, contiguous=False)
     _need(k_pool, "k_pool", BF16)
     _need(v_pool, "v_pool", BF16)
@@ -327,14 +350,21 @@ def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         _need(out, "out", BF16)
         if out.shape != q.shape:
             raise ValueError("out must have q's shape")
-    _same_device(q, k_pool=k_pool, v_pool=v_pool, block_table=block_table, cu_q=cu_q, kv_len=kv_len, out=out)
+    if workspace is not None:
+        _need(workspace, "workspace", torch.uint8)
+    elif plan_ready:
+        raise ValueError("plan_ready needs the workspace that holds the plan")
+    _same_device(q, k_pool=k_pool, v_pool=v_pool, block_table=block_table, cu_q=cu_q, kv_len=kv_len, out=out,
+                 workspace=workspace)
     with torch.cuda.device(q.device):
         if out is None:
             out = torch.empty(T, Hq, hd, dtype=BF16, device=q.device)
+        if workspace is None:
+            workspace = torch.empty(chunk_workspace_bytes(B, T, Hq, Hkv, hd), dtype=torch.uint8, device=q.device)
         _lib.call("mb_chunk_attention", _p(q), q.stride(0) if T > 1 else Hq * hd, _p(k_pool), _p(v_pool), P,
                   _p(block_table), block_table.shape[1], _p(cu_q), _p(kv_len), B, T, Hq, Hkv, hd, page, float(scale),
-                  _p(out), _stream(q))
-    _count()
+                  int(plan_ready), _p(out), _p(workspace), workspace.numel(), _stream(q))
+    _count(1 if plan_ready else 2)
     return out
 
 

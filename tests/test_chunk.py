@@ -40,9 +40,9 @@ def test_chunk_meta_refusals(lib, bad):
 
 
 def _attention(lib, q=P, q_stride=16 * 128, k=P, v=P, num_pages=8, table=P, max_pages=4, cu_q=P, kv_len=P, batch=2,
-               tokens=5, q_heads=16, kv_heads=8, head_dim=128, page=128, scale=0.1, out=P):
+               tokens=5, q_heads=16, kv_heads=8, head_dim=128, page=128, scale=0.1, out=P, ws=P, ws_bytes=1 << 30):
     return lib.mb_chunk_attention(q, q_stride, k, v, num_pages, table, max_pages, cu_q, kv_len, batch, tokens, q_heads,
-                                  kv_heads, head_dim, page, scale, out, None)
+                                  kv_heads, head_dim, page, scale, 0, out, ws, ws_bytes, None)
 
 
 @pytest.mark.parametrize("bad,code", [
@@ -51,16 +51,40 @@ def _attention(lib, q=P, q_stride=16 * 128, k=P, v=P, num_pages=8, table=P, max_
     (dict(q=None), 1), (dict(k=None), 1), (dict(v=None), 1), (dict(table=None), 1), (dict(cu_q=None), 1),
     (dict(kv_len=None), 1), (dict(out=None), 1), (dict(q=ODD), 1), (dict(k=ODD), 1), (dict(v=ODD), 1),
     (dict(out=ODD), 1), (dict(q_stride=16 * 128 - 8), 1), (dict(q_stride=16 * 128 + 4), 1),
-    (dict(num_pages=1 << 22), 2), (dict(max_pages=1 << 25), 2),
+    (dict(num_pages=1 << 22), 2), (dict(max_pages=1 << 25), 2), (dict(q_heads=258, kv_heads=2, q_stride=1 << 16), 2),
+    (dict(scale=0.0), 1), (dict(scale=-0.1), 1), (dict(scale=float("nan")), 1), (dict(scale=float("inf")), 1),
+    (dict(ws=None), 3), (dict(ws=ODD), 3), (dict(ws_bytes=1000), 3),
 ])
 def test_chunk_attention_refusals(lib, bad, code):
     assert _attention(lib, **bad) == code
     assert lib.mb_last_error()
 
 
+def _plan(lib, cu_q=P, kv_len=P, batch=2, tokens=5, q_heads=16, kv_heads=8, head_dim=128, page=128, max_pages=4, ws=P,
+          ws_bytes=1 << 30):
+    return lib.mb_chunk_plan(cu_q, kv_len, batch, tokens, q_heads, kv_heads, head_dim, page, max_pages, ws, ws_bytes, None)
+
+
+@pytest.mark.parametrize("bad,code", [
+    (dict(batch=-1), 1), (dict(tokens=-1), 1), (dict(q_heads=12), 1), (dict(head_dim=80), 2), (dict(page=32), 2),
+    (dict(cu_q=None), 1), (dict(kv_len=None), 1), (dict(max_pages=0), 1), (dict(max_pages=1 << 25), 2),
+    (dict(ws=None), 3), (dict(ws=ODD), 3), (dict(ws_bytes=1000), 3), (dict(q_heads=258, kv_heads=2), 2),
+])
+def test_chunk_plan_refusals(lib, bad, code):
+    assert _plan(lib, **bad) == code
+    assert lib.mb_last_error()
+
+
+def test_chunk_workspace_size_rules(lib):
+    size = lib.mb_chunk_workspace_bytes
+    assert 0 < size(1, 1, 16, 8, 128) < size(256, 256, 16, 8, 128) <= size(256, 6000, 16, 8, 128)
+    for bad in ((0, 1, 16, 8, 128), (1, 0, 16, 8, 128), (1, 1, 12, 8, 128), (1, 1, 16, 8, 96), (1, 1, 129, 1, 64)):
+        assert size(*bad) == 0
+
+
 def test_empty_chunk_attention_is_a_noop(lib):
-    assert _attention(lib, batch=0, q=None, k=None, v=None, table=None, cu_q=None, kv_len=None, out=None) == 0
-    assert _attention(lib, tokens=0, q=None, k=None, v=None, table=None, cu_q=None, kv_len=None, out=None) == 0
+    assert _attention(lib, batch=0, q=None, k=None, v=None, table=None, cu_q=None, kv_len=None, out=None, ws=None) == 0
+    assert _attention(lib, tokens=0, q=None, k=None, v=None, table=None, cu_q=None, kv_len=None, out=None, ws=None) == 0
 
 
 def test_wrappers_refuse_host_tensors():
