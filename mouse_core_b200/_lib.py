@@ -109,9 +109,9 @@ def check(rc: int, what: str) -> None:
 
 def call(name: str, *args):
     """Call ``name`` and raise ``KernelError`` on a non-zero status."""
-    fn = getattr(load(), name)
-    rc = fn(*args)
-    check(rc, name)
+    rc = getattr(_LIB or load(), name)(*args)
+    if rc:
+        check(rc, name)
 
 
 def device_status(clear: bool = True) -> int:

@@ -556,7 +556,7 @@ int mb_chunk_attention(const void* q, long long q_stride, const void* k_pool, co
     cudaError_t e = mb::launch_chunk_plan(p, lay, ws, sms, (cudaStream_t)stream);
     if (e != cudaSuccess) return cuda_fail(e, "chunk plan launch");
   }
-  cudaError_t e = mb::launch_chunk_attention(qm, sqm, km, vm, p, lay, ws, sms, (cudaStream_t)stream);
+  cudaError_t e = mb::launch_chunk_attention(qm, sqm, km, vm, p, lay, ws, sms, !plan_ready, (cudaStream_t)stream);
   return e == cudaSuccess ? MB_OK : cuda_fail(e, "chunk attention launch");
 }
 

@@ -14,9 +14,10 @@
 // sub-tiles of TS = 128 / G tokens (128 query rows) each. Every (tile,
 // kv-head) is one item over 128-key tiles of the cache; items with many key
 // tiles are split along the keys into pieces when the step has too few items
-// to fill the SMs (chunk_plan_kernel), each piece leaves (O, max, sum) in fp32
-// and the last piece to finish joins them in the pieces' order, so the result
-// does not depend on who was last.
+// to fill the SMs (chunk_plan_kernel): each piece leaves (O, max, sum) in fp32,
+// and chunk_join_kernel joins them in the pieces' order, so the result does not
+// depend on the schedule. (Joined by the last piece's CTA instead, a 256-row
+// tile in 7 pieces kept one CTA 170 us longer than the rest.)
 //
 // One persistent CTA per SM takes pieces from a counter, longest first, and
 // serves both kinds through one TMA ring, so that a rebuilt row's window runs
@@ -33,8 +34,7 @@
 //                small: warp w takes keys 16 w .. 16 w + 15 of every tile with
 //                mma.sync, its own running max and sum
 //   warps 12-15  epilogue: big tiles' O out of tensor memory, small tiles' join
-//                over the eight warps, the output or the piece's partial, and
-//                the join over pieces
+//                over the eight warps; the output or the piece's partial
 // Bounds: single tokens are bound by HBM (a 16-row tile needs 64 KB of K/V per
 // 128 keys), chunks by the softmax's exponentials and the tensor pipe.
 //
@@ -56,274 +56,269 @@ namespace mb {
 struct ChunkEntry {
   int4 a, b, c;
 };
+// Up to eight query rows of a split tile, for the join: the tile's first
+// partial slot, its pieces, its first token, the first of the rows, and the
+// tile's rows.
+struct alignas(16) ChunkSplit {
+  int slot, pieces, q0;
+  short row0, rows;
+};
+constexpr int kJoinRows = 8;
 
 constexpr int kChunkKeys = 128;      // keys per tile
 constexpr int kChunkSmallRows = 16;  // query rows of a small tile (one mma.sync row block)
 constexpr int kChunkPlanThreads = 1024;
-constexpr int kChunkBuckets = 2048;  // key-tile counts up to 2046 exactly, longer ones together
 // Shortest piece: below it a piece's own cost (its queries, its partial, the
 // join) outweighs what another SM gains.
 constexpr int kMinSplitTiles = 4;
+// ... and nothing is gained by pieces shorter than this part of an SM's share of
+// the step: longest first already evens those out.
+constexpr int kPiecesPerShare = 3;
 
 struct ChunkPlanParams {
   const int32_t* cu_q;
   const int32_t* kv_len;
   int batch, tokens, G, Hkv, tile_tokens, key_limit, sms, max_entries, max_slots;
   ChunkEntry* entries;
-  int* head;      // [0] entries, [1] next item, [2] CTAs done
-  int* counters;  // [max_slots * Hkv] pieces finished, by first slot and kv-head
+  ChunkSplit* splits;
+  int* head;  // [0] entries, [1] next item, [2] CTAs done, [3] splits
 };
 
-// Key tiles that query tile t of a row (n new tokens, len cached) visits.
-__device__ __forceinline__ int key_tiles(int n, int len, int t, int tile_tokens, int key_limit) {
-  const int end = min(n, (t + 1) * tile_tokens);
-  const int keys = min(len - n + end, key_limit);
-  return max(1, (max(keys, 0) + kChunkKeys - 1) / kChunkKeys);
+// Key tiles that query tile t of a row (n new tokens, len cached ones) visits.
+__device__ __forceinline__ int chunk_key_tiles(int n, int len, int t, bool small, int tile_tokens, int key_limit) {
+  const int end = small ? n : min(n, (t + 1) * tile_tokens);
+  return max(1, (max(min(len - n + end, key_limit), 0) + kChunkKeys - 1) / kChunkKeys);
 }
 
-// The work list of a step. Splitting: with E entries before it, the longest
-// tiles are cut into pieces of at most c key tiles, c the smallest that leaves
-// at most one wave of CTAs beyond the waves the unsplit items need anyway (so
-// the partials stay few), and never below kMinSplitTiles. Order: rows by the
-// length of their pieces, longest first; a row's tiles stay together, its last
-// (longest) first, so that they read the row's keys from L2.
+// The work list of a step, in one block with a row per thread. Splitting: with
+// E entries before it, the longest tiles are cut into pieces of at most c key
+// tiles, c the smallest that leaves at most one wave of CTAs beyond the waves
+// the unsplit items need anyway (so the partials stay few), and not below the
+// two bounds above. Order: rows by the length of their longest piece, longest
+// first; a row's tiles stay together, its last (longest) first, so that they
+// read the row's keys from L2.
 __global__ void __launch_bounds__(kChunkPlanThreads) chunk_plan_kernel(const ChunkPlanParams p) {
-  __shared__ int pre[kChunkPlanThreads + 1], n_s[kChunkPlanThreads], len_s[kChunkPlanThreads], base_s[kChunkPlanThreads];
-  __shared__ int hist[kChunkBuckets];
-  __shared__ int warp_tot[32];
-  __shared__ unsigned long long sum_s, over_s;
-  __shared__ int max_s, fits_s, slots_s;
-  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  auto bucket = [](int kt) { return min(kt, kChunkBuckets - 1); };
+  constexpr int kBuckets = kChunkPlanThreads;  // piece lengths, the longest together
+  __shared__ int hist[kBuckets], warp_tot[32], warp_max[32];
+  __shared__ int base_s[kChunkPlanThreads], n_s[kChunkPlanThreads], len_s[kChunkPlanThreads];
+  __shared__ int cu_s[kChunkPlanThreads], pre[kChunkPlanThreads + 1];
+  __shared__ unsigned long long warp_sum[32], fit_s[3];
+  __shared__ int slots_s, splits_s;
+  launch_dependents();  // the attention's CTAs set themselves up meanwhile
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, nw = blockDim.x >> 5;
+  const unsigned all = 0xffffffffu;
 
-  // Exclusive block scan of one count per thread into pre[0 .. threads].
-  auto scan = [&](int v) {
-    int x = v;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, d);
-      if (lane >= d) x += y;
-    }
-    __syncthreads();
-    if (lane == 31) warp_tot[w] = x;
-    __syncthreads();
-    if (w == 0) {
-      int t = warp_tot[lane];
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, t, d);
-        if (lane >= d) t += y;
-      }
-      warp_tot[lane] = t;
-    }
-    __syncthreads();
-    pre[tid + 1] = x + (w > 0 ? warp_tot[w - 1] : 0);
-    if (tid == 0) pre[0] = 0;
-    __syncthreads();
-  };
-  auto tiles_of = [&](int n) {
-    return n <= 0 ? 0 : (long long)n * p.G <= kChunkSmallRows ? 1 : (n + p.tile_tokens - 1) / p.tile_tokens;
-  };
-  // Rows r0 .. r0 + threads - 1 into n_s, len_s and the tile prefix.
-  int held = -1;
-  auto load_rows = [&](int r0) {
-    if (held == r0) return;
-    held = r0;
-    int n = 0, len = 0;
+  // Row r0 + tid: its tokens, keys and tiles.
+  int r0 = -1, n = 0, len = 0, tiles = 0, cu = 0;
+  bool small = false;
+  auto load = [&](int at) {
+    if (at == r0) return;
+    r0 = at;
+    n = len = tiles = 0;
     if (r0 + tid < p.batch) {
-      const int lo = min(max(p.cu_q[r0 + tid], 0), p.tokens);
-      n = min(max(p.cu_q[r0 + tid + 1], lo), p.tokens) - lo;
+      cu = min(max(p.cu_q[r0 + tid], 0), p.tokens);
+      n = min(max(p.cu_q[r0 + tid + 1], cu), p.tokens) - cu;
       len = max(p.kv_len[r0 + tid], 0);
-      if (n > 0 && len > p.key_limit) report(kDevBadPage);
+      small = n <= kChunkSmallRows / p.G;
+      tiles = n <= 0 ? 0 : small ? 1 : (n + p.tile_tokens - 1) / p.tile_tokens;
     }
-    __syncthreads();
-    n_s[tid] = n;
-    len_s[tid] = len;
-    scan(tiles_of(n));
   };
-  auto row_of = [&](int x) {
-    int lo = 0, hi = kChunkPlanThreads - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (pre[mid] <= x)
-        lo = mid;
-      else
-        hi = mid - 1;
-    }
-    return lo;
+  auto key_tiles = [&](int t) { return chunk_key_tiles(n, len, t, small, p.tile_tokens, p.key_limit); };
+  auto warp_add = [&](unsigned long long v) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(all, v, d);
+    return v;
   };
 
-  // 1. Histogram of the tiles' key-tile counts.
-  for (int i = tid; i < kChunkBuckets; i += kChunkPlanThreads) hist[i] = 0;
-  if (tid == 0) {
-    sum_s = over_s = 0;
-    max_s = slots_s = 0;
+  // 1. Entries, key tiles and the most of one entry, over all rows.
+  if (tid < 3) fit_s[tid] = 0;
+  if (tid == 0) slots_s = splits_s = 0;
+  hist[tid] = 0;
+  for (int i = tid + blockDim.x; i < kBuckets; i += blockDim.x) hist[i] = 0;
+  unsigned long long count = 0, sum = 0;
+  int most = 0;
+  for (int at = 0; at < p.batch; at += blockDim.x) {
+    load(at);
+    if (n > 0 && len > p.key_limit) report(kDevBadPage);
+    count += tiles;
+    for (int t = 0; t < tiles; ++t) sum += key_tiles(t);
+    if (tiles > 0) most = max(most, key_tiles(tiles - 1));
+  }
+  count = warp_add(count);
+  sum = warp_add(sum);
+  most = __reduce_max_sync(all, most);
+  if (lane == 0) {
+    warp_tot[w] = (int)min(count, 0x7fffffffull);
+    warp_sum[w] = sum;
+    warp_max[w] = most;
   }
   __syncthreads();
-  long long E = 0;
-  for (int r0 = 0; r0 < p.batch; r0 += kChunkPlanThreads) {
-    load_rows(r0);
-    const int tiles = pre[kChunkPlanThreads];
-    E += tiles;
-    unsigned long long sum = 0, over = 0;
-    int most = 0;
-    for (int x = tid; x < tiles; x += kChunkPlanThreads) {
-      const int r = row_of(x);
-      const int kt = key_tiles(n_s[r], len_s[r], x - pre[r], p.tile_tokens, p.key_limit);
-      atomicAdd(&hist[bucket(kt)], 1);
-      sum += kt;
-      if (kt >= kChunkBuckets - 1) over += kt;
-      most = max(most, kt);
-    }
-    if (sum) {
-      atomicAdd(&sum_s, sum);
-      if (over) atomicAdd(&over_s, over);
-      atomicMax(&max_s, most);
-    }
-  }
-  __syncthreads();
-  const int most = max_s;
-  // 2. The piece length c: 32 candidates a round, one per warp.
+  const long long E = (long long)warp_add(lane < nw ? (unsigned long long)warp_tot[lane] : 0);
+  sum = warp_add(lane < nw ? warp_sum[lane] : 0);
+  most = __reduce_max_sync(all, lane < nw ? warp_max[lane] : 0);
+  // 2. The piece length c, by bisection.
   const long long waves = (E * p.Hkv + p.sms - 1) / p.sms + 1;
   const long long room = waves * p.sms / p.Hkv;  // entries allowed after splitting
-  int c = max(most, 1);
+  int hi = max(most, 1);                           // splits nothing, which always fits
+  int lo = hi;
   if (room > E) {
-    int lo = (int)min((unsigned long long)c, max((sum_s + room - 1) / (unsigned long long)room,
-                                                 (unsigned long long)kMinSplitTiles));
-    int hi = c;  // c = most splits nothing, which always fits
-    while (lo < hi) {
-      const int cand = lo + (int)((long long)(hi - lo) * w / 32);
-      unsigned long long pieces = 0;
-      for (int kt = lane; kt < kChunkBuckets - 1 && kt <= most; kt += 32)
-        pieces += (unsigned long long)hist[kt] * ((kt + cand - 1) / cand);
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) pieces += __shfl_xor_sync(0xffffffffu, pieces, d);
-      pieces += over_s / cand + hist[kChunkBuckets - 1];
-      if (tid == 0) fits_s = hi;
-      __syncthreads();
-      if (lane == 0) {
-        if (pieces <= (unsigned long long)room)
-          atomicMin(&fits_s, cand);
-        warp_tot[w] = cand;
-      }
-      __syncthreads();
-      // The smallest candidate that fits bounds c from above, the one before it from below.
-      const int fit = fits_s;
-      int below = lo - 1;
-      for (int i = 0; i < 32; ++i)
-        if (warp_tot[i] < fit) below = max(below, warp_tot[i]);
-      __syncthreads();
-      hi = fit;
-      lo = below + 1;
-    }
-    c = hi;
+    const unsigned long long share = sum * p.Hkv / (kPiecesPerShare * p.sms);
+    lo = (int)min((unsigned long long)hi, max(max((sum + room - 1) / (unsigned long long)room, share),
+                                              (unsigned long long)kMinSplitTiles));
   }
-  // Pieces of a tile, and of all of a row's tiles from tile t on.
+  for (int round = 0; lo < hi; ++round) {
+    const int c = (lo + hi) >> 1;
+    unsigned long long pieces = 0;
+    for (int at = 0; at < p.batch; at += blockDim.x) {
+      load(at);
+      for (int t = 0; t < tiles; ++t) pieces += (key_tiles(t) + c - 1) / c;
+    }
+    pieces = warp_add(pieces);
+    if (lane == 0 && pieces) atomicAdd(&fit_s[round % 3], pieces);
+    if (tid == 0) fit_s[(round + 1) % 3] = 0;  // (read by nobody now: two rounds old)
+    __syncthreads();
+    if (fit_s[round % 3] <= (unsigned long long)room)
+      hi = c;
+    else
+      lo = c + 1;
+  }
+  const int c = hi;
   auto pieces_of = [&](int kt) { return kt <= c ? 1 : (kt + c - 1) / c; };
-  auto pieces_from = [&](int r, int t, int tiles) {
-    if (key_tiles(n_s[r], len_s[r], tiles - 1, p.tile_tokens, p.key_limit) <= c) return tiles - t;
+  auto row_pieces = [&]() {
+    if (tiles == 0 || key_tiles(tiles - 1) <= c) return tiles;
     int s = 0;
-    for (; t < tiles; ++t) s += pieces_of(key_tiles(n_s[r], len_s[r], t, p.tile_tokens, p.key_limit));
+    for (int t = 0; t < tiles; ++t) s += pieces_of(key_tiles(t));
     return s;
   };
-  auto sort_key = [&](int r, int tiles) {
-    const int kt = key_tiles(n_s[r], len_s[r], tiles - 1, p.tile_tokens, p.key_limit);
-    const int s = pieces_of(kt);
-    return bucket((kt + s - 1) / s);
-  };
-  // 3. Where each piece length starts in the order, longest first.
-  for (int i = tid; i < kChunkBuckets; i += kChunkPlanThreads) hist[i] = 0;
+  // Of the row's longest piece (a row with a split tile counts as c: it has
+  // pieces near it); 0 comes first.
+  auto bucket = [&]() { return kBuckets - 1 - min(min(key_tiles(tiles - 1), c), kBuckets - 1); };
+  // 3. Where each piece length starts in the order.
   __syncthreads();
-  for (int r0 = 0; r0 < p.batch; r0 += kChunkPlanThreads) {
-    load_rows(r0);
-    const int tiles = pre[tid + 1] - pre[tid];
-    if (tiles > 0) atomicAdd(&hist[sort_key(tid, tiles)], pieces_from(tid, 0, tiles));
-    __syncthreads();
+  for (int at = 0; at < p.batch; at += blockDim.x) {
+    load(at);
+    if (tiles > 0) atomicAdd(&hist[bucket()], row_pieces());
   }
-  {
-    const int i0 = kChunkBuckets - 1 - 2 * tid, i1 = i0 - 1;
-    const int h0 = hist[i0], h1 = hist[i1];
-    int x = h0 + h1;
+  __syncthreads();
+  int total = 0;
+  for (int at = 0; at < kBuckets; at += blockDim.x) {
+    const int h = hist[at + tid];
+    int x = h;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, d);
+      const int y = __shfl_up_sync(all, x, d);
       if (lane >= d) x += y;
     }
     if (lane == 31) warp_tot[w] = x;
     __syncthreads();
-    int before = x - h0 - h1;
-    for (int i = 0; i < w; ++i) before += warp_tot[i];
-    hist[i0] = before;
-    hist[i1] = before + h0;
-    if (tid == kChunkPlanThreads - 1) fits_s = before + h0 + h1;
+    int tot = lane < nw ? warp_tot[lane] : 0;
+    const int before = __reduce_add_sync(all, lane < w ? tot : 0);
+    hist[at + tid] = total + before + x - h;
+    total += __reduce_add_sync(all, tot);
     __syncthreads();
   }
-  const int total = fits_s;
   const bool fits = total <= p.max_entries;  // offsets that overlap can ask for more tiles than the stream holds
-  if (!fits && tid == 0) report(kDevBadIndex);
   if (tid == 0) {
+    if (!fits) report(kDevBadIndex);
     p.head[0] = fits ? total : 0;
     p.head[1] = p.head[2] = 0;
   }
-  for (int i = tid; i < p.max_slots * p.Hkv; i += kChunkPlanThreads) p.counters[i] = 0;
-  if (!fits) return;
-  // 4. The entries.
-  for (int r0 = 0; r0 < p.batch; r0 += kChunkPlanThreads) {
-    load_rows(r0);
-    {
-      const int tiles = pre[tid + 1] - pre[tid];
-      if (tiles > 0) base_s[tid] = atomicAdd(&hist[sort_key(tid, tiles)], pieces_from(tid, 0, tiles));
+  if (!fits) {
+    if (tid == 0) p.head[3] = 0;
+    return;
+  }
+  // 4. The entries: the group's tiles side by side, each finding its row by
+  // bisection.
+  for (int at = 0; at < p.batch; at += blockDim.x) {
+    load(at);
+    base_s[tid] = tiles > 0 ? atomicAdd(&hist[bucket()], row_pieces()) : 0;
+    n_s[tid] = n;
+    len_s[tid] = len;
+    cu_s[tid] = cu;
+    int x = tiles;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(all, x, d);
+      if (lane >= d) x += y;
     }
+    if (lane == 31) warp_tot[w] = x;
     __syncthreads();
-    for (int x = tid; x < pre[kChunkPlanThreads]; x += kChunkPlanThreads) {
-      const int r = row_of(x), t = x - pre[r], tiles = pre[r + 1] - pre[r];
-      const int n = n_s[r], len = len_s[r];
-      const bool small = (long long)n * p.G <= kChunkSmallRows;
-      const int kt = key_tiles(n, len, t, p.tile_tokens, p.key_limit);
+    const int tot = lane < nw ? warp_tot[lane] : 0;
+    pre[tid + 1] = x + __reduce_add_sync(all, lane < w ? tot : 0);
+    if (tid == 0) pre[0] = 0;
+    __syncthreads();
+    const int row0 = r0;
+    for (int e = tid; e < pre[blockDim.x]; e += blockDim.x) {
+      int r = 0, hi_r = blockDim.x - 1;
+      while (r < hi_r) {
+        const int mid = (r + hi_r + 1) >> 1;
+        if (pre[mid] <= e)
+          r = mid;
+        else
+          hi_r = mid - 1;
+      }
+      const int t = e - pre[r], last = pre[r + 1] - pre[r] - 1;
+      const int n_ = n_s[r], len_ = len_s[r];
+      const bool small_ = n_ <= kChunkSmallRows / p.G;
+      const int kt = chunk_key_tiles(n_, len_, t, small_, p.tile_tokens, p.key_limit);
       const int pieces = pieces_of(kt);
+      // Behind the row's longer tiles t + 1 .. last.
+      int first = base_s[r] + last - t;
+      if (chunk_key_tiles(n_, len_, last, small_, p.tile_tokens, p.key_limit) > c)
+        for (int u = t + 1; u <= last; ++u)
+          first += pieces_of(chunk_key_tiles(n_, len_, u, small_, p.tile_tokens, p.key_limit)) - 1;
       int slot = -1;
       if (pieces > 1) {
         slot = atomicAdd(&slots_s, pieces);
-        if (slot + pieces > p.max_slots) report(kDevBadIndex);  // cannot happen: see chunk_layout
+        if (slot + pieces > p.max_slots) {  // cannot happen: see chunk_layout
+          report(kDevBadIndex);
+          slot = -1;
+        }
       }
-      const int first = base_s[r] + pieces_from(r, t + 1, tiles);
-      const int q0 = t * p.tile_tokens;
-      const int cu = min(max(p.cu_q[r0 + r], 0), p.tokens);
-      for (int i = 0; i < pieces; ++i) {
-        const int k0 = (int)((long long)kt * i / pieces), k1 = (int)((long long)kt * (i + 1) / pieces);
-        ChunkEntry e;
-        e.a = make_int4(r0 + r, cu + q0, min(n - q0, small ? n : p.tile_tokens), len - n + q0);
-        e.b = make_int4(min(len, p.key_limit), k0, k1 - k0, slot + pieces <= p.max_slots ? slot : -1);
-        e.c = make_int4(pieces, i, small, 0);
-        p.entries[first + i] = e;
+      const int q0 = t * p.tile_tokens, ntok = small_ ? n_ : min(n_ - q0, p.tile_tokens);
+      if (slot >= 0) {
+        const int rows = ntok * p.G;
+        int at_split = atomicAdd(&splits_s, (rows + kJoinRows - 1) / kJoinRows);
+        for (int row = 0; row < rows; row += kJoinRows)
+          p.splits[at_split++] = ChunkSplit{slot, pieces, cu_s[r] + q0, (short)row, (short)rows};
+      }
+      for (int i = 0, k0 = 0; i < pieces; ++i) {
+        const int k = (kt - k0) / (pieces - i);  // even pieces
+        ChunkEntry out;
+        out.a = make_int4(row0 + r, cu_s[r] + q0, ntok, len_ - n_ + q0);
+        out.b = make_int4(min(len_, p.key_limit), k0, k, slot);
+        out.c = make_int4(pieces, i, small_, 0);
+        p.entries[first + i] = out;
+        k0 += k;
       }
     }
     __syncthreads();
   }
+  if (tid == 0) p.head[3] = splits_s;
 }
 
 // ------------------------------------------------------------- the attention
 constexpr int kChunkThreads = 512;
-constexpr int kChunkLaunchRegs = 128;  // 65536 / 512
-struct ChunkRegs {  // control, epilogue and softmax warpgroups
-  static constexpr int ctrl = 56, epi = 80, softmax = 184;
-  static_assert(128 * ctrl + 128 * epi + 256 * softmax <= kChunkThreads * kChunkLaunchRegs,
-                "the register split must fit the launch allocation");
-};
 
 template <int HD>
 struct ChunkTile {
-  static constexpr int NCB = HD / 64;               // 64-element column blocks
-  static constexpr int BOX = 128 * 128;             // bytes of a 64-element x 128-row block
-  static constexpr int QTILE = NCB * BOX;           // one sub-tile's queries
-  static constexpr int SQBOX = 16 * 128;            // a small tile's queries: 16 rows
+  static constexpr int NCB = HD / 64;             // 64-element column blocks
+  static constexpr int BOX = 128 * 128;           // bytes of a 64-element x 128-row block
+  static constexpr int QTILE = NCB * BOX;         // one sub-tile's queries
+  static constexpr int SQBOX = 16 * 128;          // a small tile's queries: 16 rows
   static constexpr int SQ = NCB * SQBOX;
-  static constexpr int KVTILE = NCB * BOX;          // one K (or V) tile
+  static constexpr int KVTILE = NCB * BOX;        // one K (or V) tile
   static constexpr int STAGES = HD == 128 ? 2 : 5;
-  static constexpr int BARS = 5632;
-  static constexpr int SMEM = 2 * QTILE + 2 * SQ + 2 * STAGES * KVTILE + BARS + 1024;
+  static constexpr int STAGE_OUT = 4 * 32 * 128;  // epilogue: 32 rows x 128 bytes per warp
+  static constexpr int BARS = 6144;
+  static constexpr int SMEM = 2 * QTILE + 2 * SQ + 2 * STAGES * KVTILE + STAGE_OUT + BARS + 1024;
   static_assert(8 * kChunkSmallRows * HD * 4 <= 2 * QTILE, "the small tiles' join lies in the big tiles' Q");
   static_assert(SMEM <= 232448, "shared memory of a CTA");
+  // Tensor memory: S of both sub-tiles, then O. With head_dim 64 there is room
+  // for P beside S, so that the next S = Q K^T runs under a tile's exponentials;
+  // with 128 P overwrites its S.
+  static constexpr bool OWN_P = HD == 64;
+  static constexpr uint32_t T_O = 256, T_P = OWN_P ? 384 : 0, P_STEP = OWN_P ? 64 : 128;
 };
 
 constexpr int kChunkMaxStages = 5;
@@ -339,25 +334,38 @@ struct ChunkWork {
 
 struct ChunkShared {
   uint64_t work_full[2], work_empty[2];   // descriptor ring (producer -> everyone)
-  uint64_t q_full[2], q_empty[2];         // by piece parity; q_empty: Q and the join area are free again
+  uint64_t q_full[2][2], q_empty[2][2];   // by piece parity and sub-tile; q_empty: its Q, or the join area, is free
   uint64_t k_full[kChunkMaxStages], v_full[kChunkMaxStages], kv_empty[kChunkMaxStages];
   uint64_t v_tail[kChunkMaxStages];       // a V tile with rows behind the last token has landed (by such tile)
   uint64_t small_done[kChunkMaxStages];   // a small tile's keys are consumed (by small tile)
-  uint64_t s_full[2], p_full[2];          // per sub-tile
-  uint64_t o_full, o_empty;
-  uint64_t stats_full[2];                 // by piece parity: max and sum (big), join area written (small)
+  uint64_t s_full[2], p_full[2][2];       // per sub-tile; P in two halves of 64 keys
+  uint64_t s_read[2], p_empty[2];         // OWN_P: S is in registers, P is consumed
+  uint64_t o_full[2], o_empty[2];         // per sub-tile
+  uint64_t stats_full[2][2];              // by piece parity and softmax warpgroup: max and sum, or join area, written
   uint64_t mma_drain;
   uint32_t tmem_base;
   int abort;                              // set by the first wait that runs out
-  int flag;                               // epilogue: this CTA joins the pieces
-  int q_armed;
+  int q_armed[2];                         // pieces whose Q loads were issued
   ChunkWork work[2];
   float stats[2][2][2][128];              // [piece parity][sub-tile][max, sum][row]; small: [.][0][.][warp * 16 + row]
 };
 static_assert(sizeof(ChunkShared) <= ChunkTile<128>::BARS, "barrier block outgrew its share");
 
-// Score of a masked key (-2^90) on the tcgen05 path, where masks are applied by
-// arithmetic; real scores stay far above it.
+// A position in a ring of N barriers and the parity of its phase.
+template <int N>
+struct ChunkRing {
+  int at = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void step() {
+    if (++at == N) {
+      at = 0;
+      phase ^= 1;
+    }
+  }
+};
+
+// Masked keys' scores lie below this (-2^90) on the tcgen05 path, where masks
+// are applied by arithmetic; real scores stay far above it.
 constexpr float kChunkMasked = -1.2379401e27f;
 
 template <int HD>
@@ -366,24 +374,32 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                            const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                            const ChunkParams p) {
   using C = ChunkTile<HD>;
+  using Ring = ChunkRing<C::STAGES>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* qs = smem;                        // [2][QTILE]; small tiles: the join area
   uint8_t* ks = qs + 2 * C::QTILE;           // [STAGES][KVTILE]
   uint8_t* vs = ks + C::STAGES * C::KVTILE;  // [STAGES][KVTILE]
   uint8_t* sq = vs + C::STAGES * C::KVTILE;  // [2][SQ]
-  ChunkShared* sh = reinterpret_cast<ChunkShared*>(sq + 2 * C::SQ);
+  uint8_t* so = sq + 2 * C::SQ;              // the epilogue's staging
+  ChunkShared* sh = reinterpret_cast<ChunkShared*>(so + C::STAGE_OUT);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
       mbar_init(&sh->work_full[s], 1);
       mbar_init(&sh->work_empty[s], 14);  // every warp but the producer and warp 3
-      mbar_init(&sh->q_full[s], 1);
-      mbar_init(&sh->q_empty[s], 1);
+      for (int t = 0; t < 2; ++t) {
+        mbar_init(&sh->q_full[s][t], 1);
+        mbar_init(&sh->q_empty[s][t], 1);
+        mbar_init(&sh->stats_full[s][t], 4);
+        mbar_init(&sh->p_full[s][t], 4);
+      }
       mbar_init(&sh->s_full[s], 1);
-      mbar_init(&sh->p_full[s], 4);
-      mbar_init(&sh->stats_full[s], 8);
+      mbar_init(&sh->s_read[s], 4);
+      mbar_init(&sh->p_empty[s], 1);
+      mbar_init(&sh->o_full[s], 1);
+      mbar_init(&sh->o_empty[s], 4);
     }
     for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(&sh->k_full[s], 1);
@@ -392,11 +408,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       mbar_init(&sh->v_tail[s], 1);
       mbar_init(&sh->small_done[s], 8);
     }
-    mbar_init(&sh->o_full, 1);
-    mbar_init(&sh->o_empty, 4);
     mbar_init(&sh->mma_drain, 1);
     sh->abort = 0;
-    sh->q_armed = 0;
+    sh->q_armed[0] = sh->q_armed[1] = 0;
     fence_barrier_init();
   }
   if (warp == 1) tmem_alloc(&sh->tmem_base, 512);
@@ -404,27 +418,34 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tbase = sh->tmem_base;
-  const int n_items = p.head[0] * p.Hkv;
+  wait_for_prior_grid();  // the plan, when it was launched just before
+  launch_dependents();    // the join waits for the SMs and then for this grid
 
   // Warp-uniform bounded wait; one that runs out stops every warp of the CTA.
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
-    return (bool)__all_sync(0xffffffffu, mbar_wait_abortable(bar, parity, code, &sh->abort));
+    return (bool)__all_sync(0xffffffffu, mbar_wait_or_abort(bar, parity, code, &sh->abort, 0));
   };
-  // Piece k of this CTA from the descriptor ring; false at the end of the work.
-  auto take = [&](int k, ChunkWork& wk) {
+  // The same off the critical path: it sleeps between polls and so leaves the
+  // issue slots to the warps at work.
+  auto sleepy = [&](uint64_t* bar, uint32_t parity) {
+    return (bool)__all_sync(0xffffffffu, mbar_wait_or_abort(bar, parity, kDevTimeoutFull, &sh->abort, 128));
+  };
+  // Piece k of this CTA from the descriptor ring (h < 0: the end of the work);
+  // take() is false at the end, too.
+  auto take_any = [&](int k, ChunkWork& wk) {
     if (!wait(&sh->work_full[k & 1], (k >> 1) & 1, kDevTimeoutFull)) return false;
     wk = sh->work[k & 1];
     __syncwarp();
     if (lane == 0) mbar_arrive(&sh->work_empty[k & 1]);
-    return wk.h >= 0;
+    return true;
   };
+  auto take = [&](int k, ChunkWork& wk) { return take_any(k, wk) && wk.h >= 0; };
   // Whether key tile t of a row holding len keys has V rows to be zeroed, i.e.
   // the last 64-row box that holds a key is not full (a box without keys is
   // loaded as zeros). Such a tile's V lands on v_tail; warp 2 completes v_full.
   auto ragged = [](int t, int len) { return len % 64 != 0 && t == len / kChunkKeys; };
 
   if (warp < 4) {
-    regs_dec<ChunkRegs::ctrl>();
     if (warp == 0) {
       // ---------------------------------------------------------- producer
       if (lane == 0) {
@@ -433,7 +454,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         prefetch_tensormap(&kmap);
         prefetch_tensormap(&vmap);
       }
-      // The next piece is taken and its entry read while this one's keys stream.
+      const int n_items = p.head[0] * p.Hkv;
+      // The next piece is taken, and its entry read, when this one's last tiles
+      // are loaded: early enough to hide the reads, late enough that a CTA
+      // busy with a long piece does not hold on to another.
       int next = 0;
       ChunkEntry e{};
       auto fetch = [&](int k) {
@@ -443,11 +467,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       };
       fetch(0);
       bool ok = true;
-      int J = 0, jc = 0;         // K/V tiles issued, those with V rows to be zeroed
-      uint32_t tails = 0;        // bit i: the tile issued i tiles ago was one of them
+      Ring kv, tail_at;
+      int issued = 0, tails_issued = 0;  // K/V tiles, and those with V rows to be zeroed
+      uint32_t tails = 0;                // bit i: the tile issued i tiles ago was one of them
       for (int k = 0;; ++k) {
-        ok = wait(&sh->work_empty[k & 1], ((k >> 1) & 1) ^ 1, kDevTimeoutEmpty);
-        if (!ok) break;
+        if (!(ok = wait(&sh->work_empty[k & 1], ((k >> 1) & 1) ^ 1, kDevTimeoutEmpty))) break;
         if (next >= n_items) {
           if (lane == 0) {
             sh->work[k & 1].h = -1;
@@ -468,45 +492,47 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         wk.pieces = e.c.x;
         wk.piece = e.c.y;
         wk.small = e.c.z;
+        wk.n0 = wk.n;
+        wk.n1 = 0;
         if (wk.ntok > p.sub_tokens && !wk.small) {
           const int keys0 = min(wk.pos0 + p.sub_tokens, p.key_limit);
-          const int end0 = max(1, (max(keys0, 0) + kChunkKeys - 1) / kChunkKeys);
-          wk.n0 = min(max(end0 - wk.k0, 0), wk.n);
+          wk.n0 = min(max(max(1, (max(keys0, 0) + kChunkKeys - 1) / kChunkKeys) - wk.k0, 0), wk.n);
           wk.n1 = wk.n;
-        } else {
-          wk.n0 = wk.n;
-          wk.n1 = 0;
         }
         if (lane == 0) {
           sh->work[k & 1] = wk;
           mbar_arrive(&sh->work_full[k & 1]);
         }
-        // Q: the small buffer of this parity is free once piece k - 2 is done,
-        // the big one (the small pieces' join area) once piece k - 1 is.
-        if (k >= 2) ok = wait(&sh->q_empty[k & 1], ((k >> 1) & 1) ^ 1, kDevTimeoutEmpty);
-        if (ok && !wk.small && k >= 1) ok = wait(&sh->q_empty[(k - 1) & 1], ((k - 1) >> 1) & 1, kDevTimeoutEmpty);
-        if (!ok) break;
-        if (lane == 0) {
-          if (wk.small) {
-            mbar_arrive_expect_tx(&sh->q_full[k & 1], C::NCB * p.small_rows * 128);
-            for (int cb = 0; cb < C::NCB; ++cb)
-              tma_load_3d(sq + (k & 1) * C::SQ + cb * C::SQBOX, &sqmap, &sh->q_full[k & 1], cb * 64, wk.h * p.G, wk.q0);
-          } else {
-            const int subs = wk.n1 > 0 ? 2 : 1;
-            mbar_arrive_expect_tx(&sh->q_full[k & 1], subs * C::NCB * p.sub_tokens * p.G * 128);
-            for (int s = 0; s < subs; ++s)
-              for (int cb = 0; cb < C::NCB; ++cb)
-                tma_load_3d(qs + s * C::QTILE + cb * C::BOX, &qmap, &sh->q_full[k & 1], cb * 64, wk.h * p.G,
-                            wk.q0 + s * p.sub_tokens);
+        // Q: the small buffer of this parity is free once piece k - 2 is done, a
+        // sub-tile's (the small pieces' join area) once piece k - 1 is. The
+        // second sub-tile's is loaded behind the first K/V tile, whose stage is
+        // free earlier.
+        auto load_q = [&](int s) {
+          const int par = wk.small ? k & 1 : (k - 1) & 1;
+          const uint32_t phase = wk.small ? ((k >> 1) & 1) ^ 1 : ((k - 1) >> 1) & 1;
+          if (k >= (wk.small ? 2 : 1) && !wait(&sh->q_empty[par][s], phase, kDevTimeoutEmpty)) return false;
+          if (wk.small && k >= 2 && !wait(&sh->q_empty[par][1], phase, kDevTimeoutEmpty)) return false;
+          if (lane == 0) {
+            uint64_t* bar = &sh->q_full[k & 1][s];
+            mbar_arrive_expect_tx(bar, C::NCB * (wk.small ? p.small_rows : p.sub_tokens * p.G) * 128);
+#pragma unroll
+            for (int cb = 0; cb < C::NCB; ++cb) {
+              uint8_t* dst = wk.small ? sq + (k & 1) * C::SQ + cb * C::SQBOX : qs + s * C::QTILE + cb * C::BOX;
+              tma_load_3d(dst, wk.small ? &sqmap : &qmap, bar, cb * 64, wk.h * p.G, wk.q0 + s * p.sub_tokens);
+            }
+            *reinterpret_cast<volatile int*>(&sh->q_armed[s]) = k + 1;
           }
-          *reinterpret_cast<volatile int*>(&sh->q_armed) = k + 1;
+          return true;
+        };
+        if (!(ok = load_q(0))) break;
+        if (wk.n1 == 0 && lane == 0) {  // nothing to load: both advance with every piece
+          mbar_arrive(&sh->q_full[k & 1][1]);
+          *reinterpret_cast<volatile int*>(&sh->q_armed[1]) = k + 1;
         }
-        fetch(k + 1);
         // K/V tiles. Page ids of the next 32 boxes at a time, one per lane.
         const int32_t* table = p.block_table + (size_t)row * p.max_pages;
         int y_lane = 0;
-        int j = 0;
-        for (; j < wk.n; ++j) {
+        for (int j = 0; j < wk.n; ++j) {
           if (j % 16 == 0) {
             const long long tok = ((long long)wk.k0 + j) * kChunkKeys + lane * 64;
             y_lane = -64;  // wholly out of bounds: reads zeros
@@ -519,42 +545,49 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 report(kDevBadPage);
             }
           }
+          if (j == max(wk.n - 2, 0)) fetch(k + 1);
           const int y0 = __shfl_sync(0xffffffffu, y_lane, 2 * (j % 16));
           const int y1 = __shfl_sync(0xffffffffu, y_lane, 2 * (j % 16) + 1);
-          const int st = (J + j) % C::STAGES;
-          if (!(ok = wait(&sh->kv_empty[st], (((J + j) / C::STAGES) & 1) ^ 1, kDevTimeoutEmpty))) break;
+          if (!(ok = wait(&sh->kv_empty[kv.at], kv.phase ^ 1, kDevTimeoutEmpty))) break;
           const bool tail = ragged(wk.k0 + j, wk.len);
           if (lane == 0) {
-            mbar_arrive_expect_tx(&sh->k_full[st], C::KVTILE);
+            uint64_t* bar = &sh->k_full[kv.at];
+            const CUtensorMap* map = &kmap;
+            uint8_t* dst = ks + kv.at * C::KVTILE;
+#pragma unroll 1
+            for (int i = 0; i < 2; ++i) {
+              mbar_arrive_expect_tx(bar, C::KVTILE);
 #pragma unroll
-            for (int cb = 0; cb < C::NCB; ++cb) {
-              uint8_t* dst = ks + st * C::KVTILE + cb * C::BOX;
-              tma_load_2d(dst, &kmap, &sh->k_full[st], cb * 64, y0);
-              tma_load_2d(dst + C::BOX / 2, &kmap, &sh->k_full[st], cb * 64, y1);
-            }
-            uint64_t* v_bar = tail ? &sh->v_tail[jc % C::STAGES] : &sh->v_full[st];
-            mbar_arrive_expect_tx(v_bar, C::KVTILE);
-#pragma unroll
-            for (int cb = 0; cb < C::NCB; ++cb) {
-              uint8_t* dst = vs + st * C::KVTILE + cb * C::BOX;
-              tma_load_2d(dst, &vmap, v_bar, cb * 64, y0);
-              tma_load_2d(dst + C::BOX / 2, &vmap, v_bar, cb * 64, y1);
+              for (int cb = 0; cb < C::NCB; ++cb) {
+                tma_load_2d(dst + cb * C::BOX, map, bar, cb * 64, y0);
+                tma_load_2d(dst + cb * C::BOX + C::BOX / 2, map, bar, cb * 64, y1);
+              }
+              bar = tail ? &sh->v_tail[tail_at.at] : &sh->v_full[kv.at];
+              map = &vmap;
+              dst = vs + kv.at * C::KVTILE;
             }
           }
-          jc += tail;
-          tails = tails << 1 | (uint32_t)tail;
           __syncwarp();
+          kv.step();
+          ++issued;
+          if (tail) {
+            tail_at.step();
+            ++tails_issued;
+          }
+          tails = tails << 1 | (uint32_t)tail;
+          if (j == 0 && wk.n1 > 0 && !(ok = load_q(1))) break;
         }
-        J += j;
         if (!ok) break;
       }
       if (lane == 0) {
         // Every load issued lands before the CTA exits, also when a wait ran out.
-        drain_ring(sh->q_full, 2, *reinterpret_cast<volatile int*>(&sh->q_armed));
-        drain_ring(sh->k_full, C::STAGES, J);
-        drain_ring(sh->v_tail, C::STAGES, jc);
-        for (int i = max(J - C::STAGES, 0); i < J; ++i)
-          if (!(tails >> (J - 1 - i) & 1)) mbar_drain(&sh->v_full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1);
+        for (int s = 0; s < 2; ++s)
+          for (int n = *reinterpret_cast<volatile int*>(&sh->q_armed[s]), i = max(n - 2, 0); i < n; ++i)
+            mbar_drain(&sh->q_full[i & 1][s], (uint32_t)(i >> 1) & 1);
+        drain_ring(sh->k_full, C::STAGES, issued);
+        drain_ring(sh->v_tail, C::STAGES, tails_issued);
+        for (int i = max(issued - C::STAGES, 0); i < issued; ++i)
+          if (!(tails >> (issued - 1 - i) & 1)) mbar_drain(&sh->v_full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1);
         // The last CTA resets the counters: the plan serves the next layer too.
         __threadfence();
         if (atomicAdd(&p.head[2], 1) == (int)gridDim.x - 1) p.head[1] = p.head[2] = 0;
@@ -564,6 +597,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       constexpr uint32_t ID_QK = umma_idesc_bf16(128, 128, 0, 0);
       constexpr uint32_t ID_PV = umma_idesc_bf16(128, HD, 0, 1);
       auto issue_qk = [&](int s, int st) {
+        tc_fence_after();
         const uint64_t dq = umma_desc_sw128(smem_u32(qs + s * C::QTILE), 16, 1024);
         const uint64_t dk = umma_desc_sw128(smem_u32(ks + st * C::KVTILE), 16, 1024);
         if constexpr (HD == 128)
@@ -572,67 +606,116 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           umma_ss_k64_warp(tbase + 128 * s, dq, dk, ID_QK);
         umma_commit_warp(&sh->s_full[s]);
       };
-      bool ok = true;
       ChunkWork wk;
-      // Running counts: K/V tiles, small tiles, each sub-tile's S tiles, big pieces.
-      int J = 0, js = 0, jb[2] = {0, 0}, big = 0;
-      for (int k = 0; ok && take(k, wk); ++k) {
+      Ring kv, small_at;
+      uint32_t tile_par = 0, o_par = 3;  // bit s: parity of sub-tile s's next P, of its O's last release
+      bool early = false;  // this piece's first S of sub-tile 0 is under way already
+      bool ok = take(0, wk);
+      for (int k = 0; ok;) {
         if (wk.small) {
-          for (int j = 0; ok && j < wk.n; ++j, ++js) {
-            ok = wait(&sh->small_done[js % C::STAGES], (js / C::STAGES) & 1, kDevTimeoutFull);
-            if (ok && lane == 0) mbar_arrive(&sh->kv_empty[(J + j) % C::STAGES]);
+          for (int j = 0; j < wk.n; ++j, kv.step(), small_at.step()) {
+            if (!(ok = wait(&sh->small_done[small_at.at], small_at.phase, kDevTimeoutFull))) break;
+            if (lane == 0) mbar_arrive(&sh->kv_empty[kv.at]);
           }
-          J += wk.n;
+          ok = ok && take(++k, wk);
           continue;
         }
-        const int n_sub[2] = {wk.n0, wk.n1};
-        if (!(ok = wait(&sh->q_full[k & 1], (k >> 1) & 1, kDevTimeoutFull))) break;
-        if (!(ok = wait(&sh->k_full[J % C::STAGES], (J / C::STAGES) & 1, kDevTimeoutFull))) break;
-        tc_fence_after();
-        for (int s = 0; s < 2; ++s)
-          if (n_sub[s] > 0) issue_qk(s, J % C::STAGES);
-        if (wk.n == 1) umma_commit_warp(&sh->q_empty[k & 1]);  // the piece's last Q K^T
-        for (int j = 0; ok && j < wk.n; ++j) {
-          const int jj = J + j, st = jj % C::STAGES, st1 = (jj + 1) % C::STAGES;
-          if (!(ok = wait(&sh->v_full[st], (jj / C::STAGES) & 1, kDevTimeoutFull))) break;
-          bool k_next = false;
-          const uint64_t dv = umma_desc_sw128(smem_u32(vs + st * C::KVTILE), C::BOX, 1024);
-          for (int s = 0; s < 2; ++s) {
-            if (j >= n_sub[s]) continue;
-            if (!(ok = wait(&sh->p_full[s], (jb[s] + j) & 1, kDevTimeoutFull))) break;
-            // The piece's first P V overwrites O: the previous epilogue must hold it.
-            if (j == 0 && big > 0 && !(ok = wait(&sh->o_empty, (big - 1) & 1, kDevTimeoutFull))) break;
-            tc_fence_after();
-            umma_ts_t128_linear_warp(tbase + 256 + HD * s, tbase + 128 * s, dv, ID_PV, j > 0 ? 1u : 0u);
-            if (j + 1 < n_sub[s]) {
-              if (!k_next && !(ok = wait(&sh->k_full[st1], ((jj + 1) / C::STAGES) & 1, kDevTimeoutFull))) break;
-              k_next = true;
-              issue_qk(s, st1);
-            }
+#pragma unroll 1
+        for (int s = early ? 1 : 0; s < 2; ++s) {
+          const int n_s = s == 0 ? wk.n0 : wk.n1;
+          // (Q is waited for even when this piece has no key for the sub-tile: it must have landed.)
+          if (!(ok = wait(&sh->q_full[k & 1][s], (k >> 1) & 1, kDevTimeoutFull))) break;
+          if (n_s > 0) {
+            if (!(ok = wait(&sh->k_full[kv.at], kv.phase, kDevTimeoutFull))) break;
+            issue_qk(s, kv.at);
           }
-          if (!ok) break;
-          if (j + 2 == wk.n) umma_commit_warp(&sh->q_empty[k & 1]);
-          umma_commit_warp(&sh->kv_empty[st]);
+          if (n_s <= 1) umma_commit_warp(&sh->q_empty[k & 1][s]);  // its last Q K^T
         }
         if (!ok) break;
-        umma_commit_warp(&sh->o_full);
-        J += wk.n;
-        jb[0] += wk.n0;
-        jb[1] += wk.n1;
-        ++big;
+        early = false;
+        ChunkWork nx;
+        nx.h = -1;
+        for (int j = 0; j < wk.n; ++j) {
+          Ring kv1 = kv;
+          kv1.step();
+          const uint64_t dv = umma_desc_sw128(smem_u32(vs + kv.at * C::KVTILE), C::BOX, 1024);
+#pragma unroll 1
+          for (int s = 0; s < 2; ++s) {
+            const int n_s = s == 0 ? wk.n0 : wk.n1;
+            if (j >= n_s) continue;
+            const uint32_t par = tile_par >> s & 1;
+            auto next_s = [&]() {
+              if (j + 1 >= n_s) return true;
+              if (!wait(&sh->k_full[kv1.at], kv1.phase, kDevTimeoutFull)) return false;
+              issue_qk(s, kv1.at);
+              if (j + 2 == n_s) umma_commit_warp(&sh->q_empty[k & 1][s]);
+              return true;
+            };
+            if (C::OWN_P && j + 1 < n_s)  // S is free once it is in registers
+              if (!(ok = wait(&sh->s_read[s], par, kDevTimeoutFull) && next_s())) break;
+            if (s == 1 && j + 1 == wk.n) {
+              // While sub-tile 1 finishes the piece, sub-tile 0 starts the next
+              // one as soon as its Q and K are there, so that the two stay out
+              // of step (in step, their exponentials compete for the same unit).
+              if (!(ok = take_any(k + 1, nx))) break;
+              const bool cand = nx.h >= 0 && !nx.small && nx.n0 > 0;
+              const uint32_t t0 = clock32();
+              while (true) {
+                if (cand && !early &&
+                    __all_sync(0xffffffffu, mbar_test_wait(&sh->q_full[(k + 1) & 1][0], ((k + 1) >> 1) & 1) &&
+                                                mbar_test_wait(&sh->k_full[kv1.at], kv1.phase))) {
+                  issue_qk(0, kv1.at);
+                  if (nx.n0 == 1) umma_commit_warp(&sh->q_empty[(k + 1) & 1][0]);
+                  early = true;
+                }
+                if (__all_sync(0xffffffffu, mbar_test_wait(&sh->p_full[1][0], par))) break;
+                if (!(ok = __all_sync(0xffffffffu, !wait_gave_up(t0, kDevTimeoutFull, &sh->abort)))) break;
+              }
+              if (!ok) break;
+            } else if (!(ok = wait(&sh->p_full[s][0], par, kDevTimeoutFull))) {
+              break;
+            }
+            if (!(ok = wait(&sh->v_full[kv.at], kv.phase, kDevTimeoutFull))) break;
+            // O += P V in two halves: the first runs under the second's
+            // exponentials. The piece's first one overwrites O, which the
+            // previous epilogue must hold.
+            if (j == 0 && !(ok = wait(&sh->o_empty[s], o_par >> s & 1, kDevTimeoutFull))) break;
+            tc_fence_after();
+            const uint32_t t_p = tbase + C::T_P + C::P_STEP * s, t_o = tbase + C::T_O + HD * s;
+            umma_ts_t64_linear_warp(t_o, t_p, dv, ID_PV, j > 0 ? 1u : 0u);
+            if (!(ok = wait(&sh->p_full[s][1], par, kDevTimeoutFull))) break;
+            tc_fence_after();
+            umma_ts_t64_linear_warp(t_o, t_p + 32, dv + 512, ID_PV, 1u);
+            if (C::OWN_P) umma_commit_warp(&sh->p_empty[s]);
+            if (j + 1 == n_s) umma_commit_warp(&sh->o_full[s]);
+            if (!C::OWN_P && !(ok = next_s())) break;
+            tile_par ^= 1u << s;
+          }
+          if (!ok) break;
+          umma_commit_warp(&sh->kv_empty[kv.at]);
+          kv = kv1;
+        }
+        if (!ok) break;
+        if (wk.n1 == 0 && !(ok = take_any(k + 1, nx))) break;
+        o_par ^= (uint32_t)(wk.n0 > 0) | (uint32_t)(wk.n1 > 0) << 1;
+        wk = nx;
+        ++k;
+        ok = wk.h >= 0;
       }
       umma_drain_warp(&sh->mma_drain);  // before TMEM is freed, also when a wait ran out
     } else if (warp == 2) {
       // ------------------------------------- zeroing behind the last token
       ChunkWork wk;
-      int J = 0, jc = 0;
-      for (int k = 0; take(k, wk); ++k) {
+      Ring tail_at;
+      int J = 0;  // tiles before this piece
+      for (int k = 0; sleepy(&sh->work_full[k & 1], (k >> 1) & 1) && take(k, wk); ++k) {
         const int j = wk.len / kChunkKeys - wk.k0;
         if (j >= 0 && j < wk.n && ragged(wk.k0 + j, wk.len)) {
           const int st = (J + j) % C::STAGES;
-          if (!wait(&sh->v_tail[jc % C::STAGES], (jc / C::STAGES) & 1, kDevTimeoutFull)) break;
+          if (!wait(&sh->v_tail[tail_at.at], tail_at.phase, kDevTimeoutFull)) break;
           const int r0 = wk.len % kChunkKeys, rows = 64 - r0 % 64;
           uint8_t* v = vs + st * C::KVTILE;
+#pragma unroll 1
           for (int i = lane; i < rows * C::NCB * 8; i += 32) {
             const int r = r0 + i / (C::NCB * 8), cb = i / 8 % C::NCB;
             *reinterpret_cast<uint4*>(v + cb * C::BOX + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
@@ -640,25 +723,26 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           fence_proxy_async();  // read by tcgen05.mma, overwritten by the next load
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh->v_full[st]);
-          ++jc;
+          tail_at.step();
         }
         J += wk.n;
       }
     }
   } else if (warp < 12) {
-    regs_inc<ChunkRegs::softmax>();
     const int hh = (warp - 4) >> 2;  // big: sub-tile
     const int sub = warp & 3;        // TMEM lane quarter this warp may access
     const int r = sub * 32 + lane;   // query row of the sub-tile
-    const int r_tok = r / p.G + hh * p.sub_tokens;
-    const bool r_in = r < p.sub_tokens * p.G;
+    const int r_tok = r < p.sub_tokens * p.G ? r / p.G + hh * p.sub_tokens : 0x7fffffff;
     const uint32_t lane_bits = (uint32_t)(sub * 32) << 16;
     const uint32_t t_s = tbase + 128 * hh + lane_bits;
-    const uint32_t t_o = tbase + 256 + HD * hh + lane_bits;
+    const uint32_t t_p = tbase + C::T_P + C::P_STEP * hh + lane_bits;
+    const uint32_t t_o = tbase + C::T_O + HD * hh + lane_bits;
     const int sw = warp - 4;  // small: its 16 keys of a tile
     const int gid = lane >> 2, tig = lane & 3;
     ChunkWork wk;
-    int J = 0, js = 0, jb = 0;
+    Ring kv, small_at;       // (kv is kept by the small pieces only, from the tile count)
+    int J = 0;               // tiles before this piece
+    uint32_t tile_par = 0;   // parity of this sub-tile's next S
     bool ok = true;
     for (int k = 0; ok && take(k, wk); ++k) {
       if (wk.small) {
@@ -670,7 +754,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           const int rr = gid + 8 * half;
           kv_end[half] = rr < R ? min(wk.pos0 + rr / p.G + 1, wk.len) : 0;
         }
-        if (!(ok = wait(&sh->q_full[k & 1], (k >> 1) & 1, kDevTimeoutFull))) break;
+        if (!(ok = wait(&sh->q_full[k & 1][0], (k >> 1) & 1, kDevTimeoutFull))) break;
         uint32_t qa[HD / 16][4];
         {
           const uint32_t qb = smem_u32(sq + (k & 1) * C::SQ);
@@ -685,12 +769,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 #pragma unroll
         for (int d = 0; d < HD / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-        for (int j = 0; j < wk.n; ++j, ++js) {
-          const int jj = J + j, st = jj % C::STAGES;
-          const int tok0 = (wk.k0 + j) * kChunkKeys + sw * 16;
-          if (!(ok = wait(&sh->k_full[st], (jj / C::STAGES) & 1, kDevTimeoutFull))) break;
+        kv.at = J % C::STAGES;
+        kv.phase = (J / C::STAGES) & 1;
+        int tok0 = wk.k0 * kChunkKeys + sw * 16;
+        for (int j = 0; j < wk.n; ++j, kv.step(), small_at.step(), tok0 += kChunkKeys) {
+          if (!(ok = wait(&sh->k_full[kv.at], kv.phase, kDevTimeoutFull))) break;
           float s[2][4];
-          const uint32_t kb = smem_u32(ks + st * C::KVTILE);
+          const uint32_t kb = smem_u32(ks + kv.at * C::KVTILE);
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
@@ -721,7 +806,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 2));
             const float m_new = fmaxf(m[half], mx[half]);
             moved |= m_new > m[half];
-            alpha[half] = m_new == -INFINITY ? 1.f : exp2f(m[half] - m_new);
+            alpha[half] = m_new == -INFINITY ? 1.f : fast_exp2(m[half] - m_new);
             m[half] = m_new;
             const float m_use = m_new == -INFINITY ? 0.f : m_new;
             l[half] *= alpha[half];
@@ -741,10 +826,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               o[d][3] *= alpha[1];
             }
           }
-          if (!(ok = wait(&sh->v_full[st], (jj / C::STAGES) & 1, kDevTimeoutFull))) break;
+          if (!(ok = wait(&sh->v_full[kv.at], kv.phase, kDevTimeoutFull))) break;
           const uint32_t pa[4] = {pack_bf16x2(s[0][0], s[0][1]), pack_bf16x2(s[0][2], s[0][3]),
                                   pack_bf16x2(s[1][0], s[1][1]), pack_bf16x2(s[1][2], s[1][3])};
-          const uint32_t vb = smem_u32(vs + st * C::KVTILE);
+          const uint32_t vb = smem_u32(vs + kv.at * C::KVTILE);
           const uint32_t rr = sw * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
 #pragma unroll
           for (int d = 0; d < HD / 8; d += 2) {
@@ -755,12 +840,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             mma_bf16_16816(o[d + 1], pa, b2, b3);
           }
           __syncwarp();
-          if (lane == 0) mbar_arrive(&sh->small_done[js % C::STAGES]);
+          if (lane == 0) mbar_arrive(&sh->small_done[small_at.at]);
         }
         if (!ok) break;
         J += wk.n;
         // Into the join area once piece k - 1 has left it.
-        if (k >= 1 && !(ok = wait(&sh->q_empty[(k - 1) & 1], ((k - 1) >> 1) & 1, kDevTimeoutEmpty))) break;
+        if (k >= 1 && !(ok = wait(&sh->q_empty[(k - 1) & 1][0], ((k - 1) >> 1) & 1, kDevTimeoutEmpty) &&
+                             wait(&sh->q_empty[(k - 1) & 1][1], ((k - 1) >> 1) & 1, kDevTimeoutEmpty)))
+          break;
         float* join = reinterpret_cast<float*>(qs) + (size_t)sw * kChunkSmallRows * HD;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -781,126 +868,156 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         }
         fence_proxy_async();  // the next big tile's Q lands here
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->stats_full[k & 1]);
+        if (lane == 0) mbar_arrive(&sh->stats_full[k & 1][hh]);
         continue;
       }
       // --------------------------------------------------- big: softmax
       const int n = hh == 0 ? wk.n0 : wk.n1;
-      const bool row_ok = r_in && r_tok < wk.ntok;
-      const int hi = row_ok ? min(wk.pos0 + r_tok, wk.len - 1) : -1;  // last visible key
+      // Last visible key. (Rows without a token compute on and are dropped.)
+      const int hi = r_tok < wk.ntok ? min(wk.pos0 + r_tok, wk.len - 1) : 0x7fffffff;
       float m_used = -INFINITY, l = 0.f;
-      for (int j = 0; j < n; ++j) {
+      for (int j = 0; j < n; ++j, tile_par ^= 1) {
         const int kv0 = (wk.k0 + j) * kChunkKeys;
-        if (!(ok = wait(&sh->s_full[hh], (jb + j) & 1, kDevTimeoutFull))) break;
+        if (!(ok = wait(&sh->s_full[hh], tile_par, kDevTimeoutFull))) break;
         tc_fence_after();
-        uint32_t v[128];
+        // S is read twice, 64 columns at a time in rolled loops: once for the
+        // maximum, once for the exponentials. (All 128 columns held in registers
+        // and unrolled, the kernel's loops outgrew the instruction cache: on
+        // short pieces, where all its roles are busy, a quarter of the fetches
+        // missed and tiles took twice as long.)
+        const bool masked = __any_sync(0xffffffffu, kv0 + kChunkKeys - 1 > hi);
+        // Keys behind the row's last visible one become hugely negative, by
+        // arithmetic: the minimum with a line that is huge up to that key and
+        // hugely negative past it (this also drops a NaN score).
+        const float big = 1.2676506e30f;  // 2^100
+        const float hb = (hi >= kv0 ? (float)min(hi - kv0, kChunkKeys - 1) + 0.5f : -1.f) * big;
+        auto load = [&](int half, uint32_t(&v)[64]) {
+          tmem_ld32(t_s + 64 * half, *reinterpret_cast<uint32_t(*)[32]>(v));
+          tmem_ld32(t_s + 64 * half + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
+          tmem_wait_ld();
+          if (masked) {
+            const float hbh = hb - (float)(64 * half) * big;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(t_s + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(v + 32 * c));
-        tmem_wait_ld();
-        if (!(row_ok && kv0 + kChunkKeys - 1 <= hi)) {
-          // Keys behind the last visible one go to kChunkMasked by arithmetic:
-          // the minimum with a line that is huge up to it and hugely negative
-          // past it (this also drops a NaN score), then the maximum with
-          // kChunkMasked.
-          const float big = 1.2676506e30f;  // 2^100
-          const float hb = (hi >= kv0 ? (float)min(hi - kv0, kChunkKeys - 1) + 0.5f : -1000.f) * big;
-#pragma unroll
-          for (int e = 0; e < 128; ++e)
-            v[e] = __float_as_uint(fmaxf(fminf(__uint_as_float(v[e]), fmaf(-(float)e, big, hb)), kChunkMasked));
-        }
-        // Row max and sum as independent chains.
-        float mp[8];
-#pragma unroll
-        for (int q = 0; q < 8; ++q) mp[q] = fmaxf(__uint_as_float(v[q]), __uint_as_float(v[8 + q]));
-#pragma unroll
-        for (int e = 16; e < 128; e += 16)
-#pragma unroll
-          for (int q = 0; q < 8; ++q) mp[q] = fmax3(mp[q], __uint_as_float(v[e + q]), __uint_as_float(v[e + 8 + q]));
-        float mx = fmax3(fmax3(mp[0], mp[1], mp[2]), fmax3(mp[3], mp[4], mp[5]), fmaxf(mp[6], mp[7]));
-        if (mx <= kChunkMasked) mx = -INFINITY;  // no key of this tile is visible to the row
-        const float m_new = fmaxf(m_used, mx * p.scale_log2);
-        // O is rescaled only when the maximum grew by more than 2^8; the final
-        // division uses the same stale maximum, so the result is exact.
-        float alpha = 1.f;
-        const bool rescale = m_new > m_used + 8.f;
-        if (rescale) {
-          alpha = exp2f(m_used - m_new);
-          m_used = m_new;
-        }
-        const float neg_mu = m_used == -INFINITY ? 0.f : -m_used;
-        float ls[8];
-#pragma unroll
-        for (int q = 0; q < 8; ++q) ls[q] = 0.f;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            float x0, x1;
-            ffma2(x0, x1, __uint_as_float(v[32 * c + e]), __uint_as_float(v[32 * c + e + 1]), p.scale_log2,
-                  p.scale_log2, neg_mu, neg_mu);
-            const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
-            const int q = 2 * ((e >> 1) & 3);
-            fadd2(ls[q], ls[q + 1], ls[q], ls[q + 1], p0, p1);
-            pk[e >> 1] = pack_bf16x2(p0, p1);
+            for (int e = 0; e < 64; ++e) v[e] = __float_as_uint(fminf(__uint_as_float(v[e]), fmaf(-(float)e, big, hbh)));
           }
-          tmem_st16(t_s + 16 * c, pk);
-        }
-        l = l * alpha + (((ls[0] + ls[1]) + (ls[2] + ls[3])) + ((ls[4] + ls[5]) + (ls[6] + ls[7])));
-        if (__any_sync(0xffffffffu, rescale && j > 0)) {
-          const float a = (rescale && j > 0) ? alpha : 1.f;
+        };
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          uint32_t v[64];
+          load(half, v);
+          float mp[8];  // independent chains
 #pragma unroll
-          for (int c = 0; c < HD / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(t_o + 32 * c, o);
+          for (int q = 0; q < 8; ++q) mp[q] = fmaxf(__uint_as_float(v[q]), __uint_as_float(v[8 + q]));
+#pragma unroll
+          for (int e = 16; e < 64; e += 16)
+#pragma unroll
+            for (int q = 0; q < 8; ++q) mp[q] = fmax3(mp[q], __uint_as_float(v[e + q]), __uint_as_float(v[e + 8 + q]));
+          mx = fmax3(fmax3(mp[0], mp[1], mp[2]), fmax3(mp[3], mp[4], mp[5]), fmax3(mp[6], mp[7], mx));
+        }
+        // O is rescaled only when the maximum grew by more than 2^8: the final
+        // division uses the same stale maximum, so the result is exact. (A row
+        // that sees no key of the tile keeps -inf.)
+        const float m_tile = mx <= kChunkMasked ? -INFINITY : mx * p.scale_log2;
+        const bool grew = m_tile > m_used + 8.f;
+        // P's columns (and O) are free once the tile before is consumed.
+        if (C::OWN_P) {
+          if (!(ok = wait(&sh->p_empty[hh], tile_par ^ 1, kDevTimeoutEmpty))) break;
+          tc_fence_after();
+        }
+        if (j == 0) {
+          m_used = m_tile;
+        } else if (__any_sync(0xffffffffu, grew)) {
+          const float alpha = grew ? fast_exp2(m_used - m_tile) : 1.f;
+          if (grew) m_used = m_tile;
+          l *= alpha;
+#pragma unroll 1
+          for (int c = 0; c < HD / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld16(t_o + 16 * c, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
-            tmem_st32(t_o + 32 * c, o);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st16(t_o + 16 * c, o);
           }
+          tmem_wait_st();
         }
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->p_full[hh]);
+        const float neg_mu = m_used == -INFINITY ? 0.f : -m_used;
+        // P and its row sums. Without P columns of its own, P's first half lies
+        // over the S columns 0 .. 31 and its second over 32 .. 63, both read.
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          uint32_t v[64];
+          load(half, v);
+          if (C::OWN_P && half == 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->s_read[hh]);
+          }
+          float ls[8];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) ls[q] = 0.f;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              float x0, x1;
+              ffma2(x0, x1, __uint_as_float(v[32 * c + e]), __uint_as_float(v[32 * c + e + 1]), p.scale_log2,
+                    p.scale_log2, neg_mu, neg_mu);
+              const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+              const int q = 2 * ((e >> 1) & 3);
+              fadd2(ls[q], ls[q + 1], ls[q], ls[q + 1], p0, p1);
+              pk[e >> 1] = pack_bf16x2(p0, p1);
+            }
+            tmem_st16(t_p + 32 * half + 16 * c, pk);
+          }
+          l += ((ls[0] + ls[1]) + (ls[2] + ls[3])) + ((ls[4] + ls[5]) + (ls[6] + ls[7]));
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->p_full[hh][half]);
+        }
       }
       if (!ok) break;
       sh->stats[k & 1][hh][0][r] = m_used;
       sh->stats[k & 1][hh][1][r] = l;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh->stats_full[k & 1]);
-      jb += n;
+      if (lane == 0) mbar_arrive(&sh->stats_full[k & 1][hh]);
       J += wk.n;
     }
   } else {
-    regs_dec<ChunkRegs::epi>();
     // ------------------------------------------------------------ epilogue
     const int tid = threadIdx.x - 384;
     const int sub = warp & 3;
     const int r = sub * 32 + lane;
     const uint32_t lane_bits = (uint32_t)(sub * 32) << 16;
-    auto sleepy = [&](uint64_t* bar, uint32_t parity) {
-      return (bool)__all_sync(0xffffffffu, mbar_wait_sleepy_abortable(bar, parity, kDevTimeoutFull, &sh->abort));
-    };
+    // Where this lane's stores of a sub-tile's turned lines go, from the
+    // sub-tile's first query row.
+    int off[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int qr = sub * 32 + i * 4 + (lane >> 3);
+      off[i] = (qr / p.G * p.Hq + qr % p.G) * HD + 8 * (lane & 7);
+    }
     ChunkWork wk;
-    int big = 0;
+    uint32_t o_par = 0;  // bit s: parity of sub-tile s's next O
+    bool ok = true;
     for (int k = 0;; ++k) {
-      // The four warps leave together: they share named barriers below.
+      // The four warps leave together: they share named barriers.
       wk.h = 0;
-      bool ok = sleepy(&sh->work_full[k & 1], (k >> 1) & 1);
-      if (ok) {
-        const bool more = take(k, wk);
-        ok = more || wk.h < 0;
-      }
+      ok = ok && sleepy(&sh->work_full[k & 1], (k >> 1) & 1);
+      if (ok) wk = sh->work[k & 1];
       if (named_barrier_or(1, 128, !ok) || wk.h < 0) break;
-      ok = sleepy(&sh->stats_full[k & 1], (k >> 1) & 1) && (wk.small || sleepy(&sh->o_full, big & 1));
-      if (named_barrier_or(1, 128, !ok)) break;
       const bool split = wk.pieces > 1;
       const int rows = wk.ntok * p.G;
       const size_t part = ((size_t)(wk.slot + wk.piece) * p.Hkv + wk.h) * p.part_rows;
       if (wk.small) {
+        ok = sleepy(&sh->stats_full[k & 1][0], (k >> 1) & 1) && sleepy(&sh->stats_full[k & 1][1], (k >> 1) & 1);
+        if (named_barrier_or(1, 128, !ok)) break;
         const float* join = reinterpret_cast<const float*>(qs);
         const float(*st)[128] = sh->stats[k & 1][0];
+#pragma unroll 1
         for (int i = tid; i < rows * (HD / 4); i += 128) {
           const int rr = i / (HD / 4), c4 = i % (HD / 4);
           float M = -INFINITY;
@@ -912,7 +1029,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           const int at = rr * HD + (((c4 >> 1) ^ (rr & 7)) * 8 + (c4 & 1) * 4);
 #pragma unroll
           for (int w = 0; w < 8; ++w) {
-            const float f = exp2f(st[0][w * 16 + rr] - Mu);
+            const float f = fast_exp2(st[0][w * 16 + rr] - Mu);
             const float4 x = *reinterpret_cast<const float4*>(&join[w * kChunkSmallRows * HD + at]);
             L += st[1][w * 16 + rr] * f;
             O.x += x.x * f;
@@ -934,92 +1051,81 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         }
         fence_proxy_async();  // the next big tile's Q lands here
         named_barrier(1, 128);
-        if (tid == 0) mbar_arrive(&sh->q_empty[k & 1]);
+        if (tid < 2) mbar_arrive(&sh->q_empty[k & 1][tid]);
       } else {
-        tc_fence_after();
+        // O out of tensor memory a row per lane, 128 bytes of it at a time,
+        // turned in shared memory so that eight lanes store a whole line.
+        uint8_t* stage = so + (warp - 12) * 4096;
+        const int sub_rows = p.sub_tokens * p.G;
+#pragma unroll 1
         for (int hh = 0; hh < 2; ++hh) {
-          const int r_tok = r / p.G + hh * p.sub_tokens;
-          const bool row_ok = r < p.sub_tokens * p.G && r_tok < wk.ntok;
           if (hh * p.sub_tokens >= wk.ntok) break;
+          const bool any = (hh == 0 ? wk.n0 : wk.n1) > 0;  // else: no key tile of this piece
+          if (!(ok = sleepy(&sh->stats_full[k & 1][hh], (k >> 1) & 1))) break;
+          if (any) {
+            if (!(ok = sleepy(&sh->o_full[hh], o_par >> hh & 1))) break;
+            o_par ^= 1u << hh;
+            tc_fence_after();
+          }
           const float m_used = sh->stats[k & 1][hh][0][r];
           const float l = sh->stats[k & 1][hh][1][r];
-          const float inv = l > 0.f ? 1.f / l : 0.f;
-          const uint32_t t_o = tbase + 256 + HD * hh + lane_bits;
-          const int tok = wk.q0 + r_tok, h = wk.h * p.G + r % p.G;
-          uint4* dst = reinterpret_cast<uint4*>(p.out + ((size_t)tok * p.Hq + h) * HD);
-          const size_t pr = part + hh * p.sub_tokens * p.G + r;
-          float4* pdst = reinterpret_cast<float4*>(p.part_o + pr * HD);
-#pragma unroll
-          for (int c = 0; c < HD / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(t_o + 32 * c, o);
-            tmem_wait_ld();
-            if (!row_ok) {
-            } else if (split) {
-#pragma unroll
-              for (int q = 0; q < 8; ++q) {
-                float4 f;
-                f.x = l > 0.f ? __uint_as_float(o[4 * q + 0]) : 0.f;
-                f.y = l > 0.f ? __uint_as_float(o[4 * q + 1]) : 0.f;
-                f.z = l > 0.f ? __uint_as_float(o[4 * q + 2]) : 0.f;
-                f.w = l > 0.f ? __uint_as_float(o[4 * q + 3]) : 0.f;
-                pdst[8 * c + q] = f;
+          const float inv = split ? 1.f : 1.f / l;
+          const uint32_t t_o = tbase + C::T_O + HD * hh + lane_bits;
+          const int live = min(sub_rows, rows - hh * sub_rows) - sub * 32;  // of this warp's 32 rows
+          const size_t pr = part + hh * sub_rows + sub * 32;
+          __nv_bfloat16* out = p.out + ((size_t)(wk.q0 + hh * p.sub_tokens) * p.Hq + wk.h * p.G) * HD;
+          const int cols = split ? 32 : 64;  // of a 128-byte line
+#pragma unroll 1
+          for (int c0 = 0; c0 < HD; c0 += cols) {
+#pragma unroll 1
+            for (int c = c0; c < c0 + cols; c += 16) {
+              uint32_t o[16];
+              tmem_ld16(t_o + c, o);
+              tmem_wait_ld();
+              if (c == HD - 16 && any) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh->o_empty[hh]);  // the next piece may overwrite O
               }
-            } else {
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                uint4 u;
-                u.x = pack_bf16x2(__uint_as_float(o[8 * q + 0]) * inv, __uint_as_float(o[8 * q + 1]) * inv);
-                u.y = pack_bf16x2(__uint_as_float(o[8 * q + 2]) * inv, __uint_as_float(o[8 * q + 3]) * inv);
-                u.z = pack_bf16x2(__uint_as_float(o[8 * q + 4]) * inv, __uint_as_float(o[8 * q + 5]) * inv);
-                u.w = pack_bf16x2(__uint_as_float(o[8 * q + 6]) * inv, __uint_as_float(o[8 * q + 7]) * inv);
-                dst[4 * c + q] = l > 0.f ? u : make_uint4(0, 0, 0, 0);
+              for (int e = 0; e < 16; ++e) o[e] = l > 0.f ? __float_as_uint(__uint_as_float(o[e]) * inv) : 0u;
+              if (split) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                  *reinterpret_cast<uint4*>(stage + lane * 128 + ((((c - c0) / 4 + q) ^ (lane & 7)) << 4)) =
+                      make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+              } else {
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                  uint4 u;
+                  u.x = pack_bf16x2(__uint_as_float(o[8 * q + 0]), __uint_as_float(o[8 * q + 1]));
+                  u.y = pack_bf16x2(__uint_as_float(o[8 * q + 2]), __uint_as_float(o[8 * q + 3]));
+                  u.z = pack_bf16x2(__uint_as_float(o[8 * q + 4]), __uint_as_float(o[8 * q + 5]));
+                  u.w = pack_bf16x2(__uint_as_float(o[8 * q + 6]), __uint_as_float(o[8 * q + 7]));
+                  *reinterpret_cast<uint4*>(stage + lane * 128 + ((((c - c0) / 8 + q) ^ (lane & 7)) << 4)) = u;
+                }
               }
             }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int row = i * 4 + (lane >> 3);
+              const uint4 u = *reinterpret_cast<const uint4*>(stage + row * 128 + (((lane & 7) ^ (row & 7)) << 4));
+              if (row >= live) continue;
+              if (split)
+                *reinterpret_cast<uint4*>(p.part_o + (pr + row) * HD + c0 + 4 * (lane & 7)) = u;
+              else
+                *reinterpret_cast<uint4*>(out + off[i] + c0) = u;
+            }
+            __syncwarp();
           }
-          if (split && row_ok) p.part_ml[pr] = make_float2(m_used, l);
+          if (split && lane < live) p.part_ml[pr + lane] = make_float2(m_used, l);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->o_empty);
-        ++big;
       }
-      if (!split) continue;
-      // Release this piece's partial and take a ticket; the last piece joins
-      // them all, in their order.
-      __threadfence();
-      named_barrier(1, 128);
-      if (tid == 0) sh->flag = atomicAdd(&p.counters[wk.slot * p.Hkv + wk.h], 1) == wk.pieces - 1;
-      named_barrier(1, 128);
-      if (!sh->flag) continue;
-      __threadfence();
-      const size_t first = ((size_t)wk.slot * p.Hkv + wk.h) * p.part_rows, step = (size_t)p.Hkv * p.part_rows;
-      for (int i = tid; i < rows * (HD / 4); i += 128) {
-        const int rr = i / (HD / 4), c4 = i % (HD / 4);
-        float M = -INFINITY;
-        for (int c = 0; c < wk.pieces; ++c) M = fmaxf(M, __ldcg(&p.part_ml[first + c * step + rr]).x);
-        const float Mu = M == -INFINITY ? 0.f : M;
-        float L = 0.f;
-        float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int c = 0; c < wk.pieces; ++c) {
-          const float2 ml = __ldcg(&p.part_ml[first + c * step + rr]);
-          const float4 x = __ldcg(reinterpret_cast<const float4*>(&p.part_o[(first + c * step + rr) * HD + c4 * 4]));
-          const float f = exp2f(ml.x - Mu);
-          L += ml.y * f;
-          O.x += x.x * f;
-          O.y += x.y * f;
-          O.z += x.z * f;
-          O.w += x.w * f;
-        }
-        const float inv = L > 0.f ? 1.f / L : 0.f;
-        const int tok = wk.q0 + rr / p.G, h = wk.h * p.G + rr % p.G;
-        uint2 u;
-        u.x = pack_bf16x2(O.x * inv, O.y * inv);
-        u.y = pack_bf16x2(O.z * inv, O.w * inv);
-        *reinterpret_cast<uint2*>(p.out + ((size_t)tok * p.Hq + h) * HD + c4 * 4) = u;
-      }
-      if (tid == 0) p.counters[wk.slot * p.Hkv + wk.h] = 0;  // ready for the next layer
+      // Only now: nobody gets two pieces ahead of the epilogue, so max, sum and
+      // join area by piece parity are enough.
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->work_empty[k & 1]);
     }
   }
   tc_fence_before();
@@ -1028,6 +1134,51 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   if (warp == 1) {
     __syncwarp();
     tmem_dealloc(tbase, 512);
+  }
+}
+
+// out of the split tiles: over a row's pieces, in their order, M = max m,
+// out = sum O 2^(m - M) / sum l 2^(m - M). A warp per row.
+template <int HD>
+__global__ void __launch_bounds__(32 * kJoinRows, 4) chunk_join_kernel(const ChunkParams p) {
+  constexpr int E = HD / 32;  // output elements per lane
+  wait_for_prior_grid();
+  const int lane = threadIdx.x & 31;
+  const int units = p.head[3] * p.Hkv;
+  const size_t step = (size_t)p.Hkv * p.part_rows;
+  for (int u = blockIdx.x; u < units; u += gridDim.x) {
+    const int h = u % p.Hkv;
+    const ChunkSplit sp = p.splits[u / p.Hkv];
+    const int row = sp.row0 + (threadIdx.x >> 5);
+    if (row >= sp.rows) continue;
+    const size_t first = ((size_t)sp.slot * p.Hkv + h) * p.part_rows + row;
+    float M = -INFINITY;
+    for (int c = lane; c < sp.pieces; c += 32) M = fmaxf(M, p.part_ml[first + c * step].x);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+    float L = 0.f, o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+    if (M > -INFINITY) {
+#pragma unroll 2
+      for (int c = 0; c < sp.pieces; ++c) {
+        const float2 ml = p.part_ml[first + c * step];
+        const float f = exp2f(ml.x - M);
+        const float* src = p.part_o + (first + c * step) * HD + lane * E;
+        L += ml.y * f;
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          const float2 x = *reinterpret_cast<const float2*>(src + e);
+          o[e] += x.x * f;
+          o[e + 1] += x.y * f;
+        }
+      }
+    }
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    __nv_bfloat16* dst = p.out + ((size_t)(sp.q0 + row / p.G) * p.Hq + h * p.G + row % p.G) * HD + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; e += 2)
+      *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16x2(o[e] * inv, o[e + 1] * inv);
   }
 }
 
@@ -1048,7 +1199,7 @@ size_t chunk_layout(int batch, int tokens, int Hq, int Hkv, int head_dim, int sm
   size_t off = 0;
   lay->head = off;     off = up(off + 4 * sizeof(int));
   lay->entries = off;  off = up(off + lay->max_entries * sizeof(ChunkEntry));
-  lay->counters = off; off = up(off + lay->max_slots * Hkv * sizeof(int));
+  lay->splits = off;   off = up(off + extra * ((lay->part_rows + kJoinRows - 1) / kJoinRows) * sizeof(ChunkSplit));
   lay->part_ml = off;  off = up(off + lay->max_slots * Hkv * lay->part_rows * sizeof(float2));
   lay->part_o = off;   off = up(off + lay->max_slots * Hkv * lay->part_rows * head_dim * sizeof(float));
   lay->total = off;
@@ -1071,50 +1222,65 @@ cudaError_t launch_chunk_plan(const ChunkParams& p, const ChunkLayout& lay, uint
   q.max_slots = (int)lay.max_slots;
   q.entries = reinterpret_cast<ChunkEntry*>(ws + lay.entries);
   q.head = reinterpret_cast<int*>(ws + lay.head);
-  q.counters = reinterpret_cast<int*>(ws + lay.counters);
-  chunk_plan_kernel<<<1, kChunkPlanThreads, 0, stream>>>(q);
+  q.splits = reinterpret_cast<ChunkSplit*>(ws + lay.splits);
+  int threads = 256;  // a power of two: the buckets are scanned in whole blocks of threads
+  while (threads < kChunkPlanThreads && threads < p.batch) threads *= 2;
+  chunk_plan_kernel<<<1, threads, 0, stream>>>(q);
   return cudaGetLastError();
 }
 
-// One-time set-up of an instantiation on the current device: its shared
-// memory, and a check that it is launched with the registers that the
-// setmaxnreg split draws on (an increase beyond them would never complete).
+// One-time set-up of an instantiation on the current device: its shared memory.
 template <int HD>
 static cudaError_t chunk_prepare() {
   static std::atomic<int> ready[kMaxDevices];
   const int dev = device_slot();
   if (dev >= 0 && ready[dev].load(std::memory_order_acquire)) return cudaSuccess;
-  cudaFuncAttributes a{};
-  cudaError_t e = cudaFuncGetAttributes(&a, chunk_attention_kernel<HD>);
-  if (e != cudaSuccess) return e;
-  if (a.numRegs < kChunkLaunchRegs) return cudaErrorInvalidConfiguration;
-  e = cudaFuncSetAttribute(chunk_attention_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           ChunkTile<HD>::SMEM);
+  cudaError_t e = cudaFuncSetAttribute(chunk_attention_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       ChunkTile<HD>::SMEM);
   if (e == cudaSuccess && dev >= 0) ready[dev].store(1, std::memory_order_release);
   return e;
 }
 
 template <int HD>
 static cudaError_t launch_chunk(const CUtensorMap& qm, const CUtensorMap& sqm, const CUtensorMap& km,
-                                const CUtensorMap& vm, const ChunkParams& p, unsigned grid, cudaStream_t stream) {
+                                const CUtensorMap& vm, const ChunkParams& p, unsigned grid, bool after_plan,
+                                cudaStream_t stream) {
   cudaError_t e = chunk_prepare<HD>();
   if (e != cudaSuccess) return e;
-  chunk_attention_kernel<HD><<<grid, kChunkThreads, ChunkTile<HD>::SMEM, stream>>>(qm, sqm, km, vm, p);
-  return cudaGetLastError();
+  // Right behind its plan the kernel starts early and waits for it in its
+  // own prologue; otherwise it is an ordinary launch.
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kChunkThreads);
+  cfg.dynamicSmemBytes = ChunkTile<HD>::SMEM;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = after_plan ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, chunk_attention_kernel<HD>, qm, sqm, km, vm, p);
+  // A table too narrow for two pieces needs no join.
+  if (e != cudaSuccess || p.key_limit <= kMinSplitTiles * kChunkKeys) return e;
+  cfg.gridDim = dim3(8 * grid);
+  cfg.blockDim = dim3(32 * kJoinRows);
+  cfg.dynamicSmemBytes = 0;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, chunk_join_kernel<HD>, p);
 }
 
 cudaError_t launch_chunk_attention(const CUtensorMap& qm, const CUtensorMap& sqm, const CUtensorMap& km,
                                    const CUtensorMap& vm, ChunkParams p, const ChunkLayout& lay, uint8_t* ws, int sms,
-                                   cudaStream_t stream) {
+                                   bool after_plan, cudaStream_t stream) {
   p.entries = reinterpret_cast<const ChunkEntry*>(ws + lay.entries);
   p.head = reinterpret_cast<int*>(ws + lay.head);
-  p.counters = reinterpret_cast<int*>(ws + lay.counters);
+  p.splits = reinterpret_cast<const ChunkSplit*>(ws + lay.splits);
   p.part_ml = reinterpret_cast<float2*>(ws + lay.part_ml);
   p.part_o = reinterpret_cast<float*>(ws + lay.part_o);
   p.part_rows = lay.part_rows;
   const unsigned grid = (unsigned)std::min<size_t>((size_t)sms, lay.max_entries * p.Hkv);
-  return p.head_dim == 128 ? launch_chunk<128>(qm, sqm, km, vm, p, grid, stream)
-                           : launch_chunk<64>(qm, sqm, km, vm, p, grid, stream);
+  return p.head_dim == 128 ? launch_chunk<128>(qm, sqm, km, vm, p, grid, after_plan, stream)
+                           : launch_chunk<64>(qm, sqm, km, vm, p, grid, after_plan, stream);
 }
 
 }  // namespace mb

@@ -13,8 +13,8 @@
 //   new_len[b]      = c_b + n_b
 //
 // Bound: launch latency below some hundred thousand tokens (8 bytes written per
-// token, 20 per row). Every block walks the rows in groups of one per thread
-// and scans (tokens, pages) itself, so one launch without a grid barrier does
+// token, 20 per row). Every block walks the rows in groups of four per
+// thread and scans (tokens, pages) itself, so one launch without a grid barrier does
 // the whole step; the tokens and opened pages of a group are spread over the
 // blocks, each token finding its row by bisection in shared memory.
 #include "common.cuh"
@@ -22,7 +22,7 @@
 
 namespace mb {
 
-constexpr int kChunkMetaThreads = 1024;
+constexpr int kChunkMetaThreads = 1024, kChunkMetaRows = 4 * kChunkMetaThreads;  // a thread scans four rows
 
 // Pages that hold n tokens.
 __device__ __forceinline__ int pages_of(int n, int page_size) { return n / page_size + (n % page_size > 0); }
@@ -34,21 +34,29 @@ __device__ __forceinline__ int add_capped(int a, int b) {
 }
 
 __global__ void __launch_bounds__(kChunkMetaThreads) chunk_meta_kernel(const ChunkMetaParams p) {
-  __shared__ int cu[kChunkMetaThreads + 1], cup[kChunkMetaThreads + 1], old_len[kChunkMetaThreads];
+  __shared__ int cu[kChunkMetaRows + 1], cup[kChunkMetaRows + 1];
   __shared__ int warp_n[32], warp_o[32];
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int first = blockIdx.x * kChunkMetaThreads + tid, stride = gridDim.x * kChunkMetaThreads;
   const int P = p.page_size;
   int base_n = 0, base_o = 0;  // tokens and pages of the groups before this one
-  for (int r0 = 0, group = 0; r0 < p.batch; r0 += kChunkMetaThreads, ++group) {
-    const int rows = min(kChunkMetaThreads, p.batch - r0);
-    int n = 0, c = 0, o = 0;
-    if (tid < rows) {
-      n = max(p.lengths[r0 + tid], 0);
-      c = max(p.kv_len[r0 + tid], 0);
-      o = pages_of(add_capped(c, n), P) - pages_of(c, P);
+  for (int r0 = 0, group = 0; r0 < p.batch; r0 += kChunkMetaRows, ++group) {
+    const int rows = min(kChunkMetaRows, p.batch - r0);
+    int n[4], c[4], o[4], sn = 0, so = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 4 * tid + i;
+      n[i] = r < rows ? max(p.lengths[r0 + r], 0) : 0;
+      c[i] = r < rows ? max(p.kv_len[r0 + r], 0) : 0;
     }
-    int sn = n, so = o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      o[i] = n[i] > 0 ? pages_of(add_capped(c[i], n[i]), P) - pages_of(c[i], P) : 0;
+      sn = add_capped(sn, n[i]);
+      so = add_capped(so, o[i]);
+    }
+    // Block scan of the threads' sums: within the warp, then every warp over
+    // the warps' totals.
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const int an = __shfl_up_sync(0xffffffffu, sn, d), ao = __shfl_up_sync(0xffffffffu, so, d);
@@ -61,42 +69,43 @@ __global__ void __launch_bounds__(kChunkMetaThreads) chunk_meta_kernel(const Chu
       warp_n[w] = sn;
       warp_o[w] = so;
     }
-    __syncthreads();  // (also: every thread has left the previous group's arrays)
-    if (w == 0) {
-      int tn = warp_n[lane], to = warp_o[lane];
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int an = __shfl_up_sync(0xffffffffu, tn, d), ao = __shfl_up_sync(0xffffffffu, to, d);
-        if (lane >= d) {
-          tn = add_capped(tn, an);
-          to = add_capped(to, ao);
-        }
-      }
-      warp_n[lane] = tn;
-      warp_o[lane] = to;
-    }
     __syncthreads();
-    sn = add_capped(base_n, add_capped(sn, w > 0 ? warp_n[w - 1] : 0));
-    so = add_capped(base_o, add_capped(so, w > 0 ? warp_o[w - 1] : 0));
-    cu[tid + 1] = sn;
-    cup[tid + 1] = so;
-    old_len[tid] = c;
+    int tn = warp_n[lane], to = warp_o[lane];
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int an = __shfl_up_sync(0xffffffffu, tn, d), ao = __shfl_up_sync(0xffffffffu, to, d);
+      if (lane >= d) {
+        tn = add_capped(tn, an);
+        to = add_capped(to, ao);
+      }
+    }
+    // Before this thread's rows: the groups, the warps and the lanes before it.
+    const int pn = __shfl_sync(0xffffffffu, tn, max(w - 1, 0)), po = __shfl_sync(0xffffffffu, to, max(w - 1, 0));
+    const int ln = __shfl_up_sync(0xffffffffu, sn, 1), lo = __shfl_up_sync(0xffffffffu, so, 1);
+    int en = add_capped(base_n, add_capped(w > 0 ? pn : 0, lane > 0 ? ln : 0));
+    int eo = add_capped(base_o, add_capped(w > 0 ? po : 0, lane > 0 ? lo : 0));
     if (tid == 0) {
       cu[0] = base_n;
       cup[0] = base_o;
     }
-    if (group % gridDim.x == blockIdx.x && tid < rows) {
-      p.cu_q[r0 + tid + 1] = sn;
-      p.cu_pages[r0 + tid + 1] = so;
-      p.new_len[r0 + tid] = add_capped(c, n);
-      if (r0 + tid == 0) {
-        p.cu_q[0] = 0;
-        p.cu_pages[0] = 0;
+    const bool mine = group % gridDim.x == blockIdx.x;  // this block writes the group's rows
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 4 * tid + i;
+      en = add_capped(en, n[i]);
+      eo = add_capped(eo, o[i]);
+      cu[r + 1] = en;
+      cup[r + 1] = eo;
+      if (mine && r < rows) {
+        p.cu_q[r0 + r + 1] = en;
+        p.cu_pages[r0 + r + 1] = eo;
+        p.new_len[r0 + r] = add_capped(c[i], n[i]);
+        // More tokens or pages than the caller gave room for: what fits is done.
+        if (en > p.tokens) report(kDevBadIndex);
+        if (eo > p.n_free || (o[i] > 0 && pages_of(c[i], P) + o[i] > p.max_pages)) report(kDevBadPage);
       }
-      // More tokens or pages than the caller gave room for: what fits is done.
-      if (sn > p.tokens) report(kDevBadIndex);
-      if (so > p.n_free || (o > 0 && pages_of(c, P) + o > p.max_pages)) report(kDevBadPage);
     }
+    if (mine && r0 == 0 && tid == 0) p.cu_q[0] = p.cu_pages[0] = 0;
     __syncthreads();
     // Row of the group that element x lies in: the last one whose prefix is <= x.
     auto row_of = [&](const int* prefix, int x) {
@@ -115,13 +124,13 @@ __global__ void __launch_bounds__(kChunkMetaThreads) chunk_meta_kernel(const Chu
     base_o = cup[rows];
     for (long long x = (long long)cup[0] + first; x < end_o; x += stride) {
       const int r = row_of(cup, (int)x);
-      const long long col = pages_of(old_len[r], P) + (x - cup[r]);
+      const long long col = pages_of(max(p.kv_len[r0 + r], 0), P) + (x - cup[r]);
       if (col < p.max_pages) p.block_table[(size_t)(r0 + r) * p.max_pages + col] = p.free_pages[x];
     }
     for (long long x = (long long)cu[0] + first; x < end_n; x += stride) {
       const int r = row_of(cu, (int)x);
-      const int pos = add_capped(old_len[r], (int)x - cu[r]);
-      const int col = pos / P, held = pages_of(old_len[r], P);
+      const int old = max(p.kv_len[r0 + r], 0), pos = add_capped(old, (int)x - cu[r]);
+      const int col = pos / P, held = pages_of(old, P);
       int id = -1;
       if (col < p.max_pages) {
         // A page opened by this step is taken from the free list again: another

@@ -95,6 +95,19 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
+// One test without suspending the thread.
+__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
 __device__ __forceinline__ long long wait_limit() {
   return *reinterpret_cast<volatile long long*>(&g_wait_limit);
 }
@@ -152,22 +165,33 @@ __device__ __forceinline__ bool mbar_wait_abortable(uint64_t* bar, uint32_t pari
   }
 }
 
-// mbar_wait_abortable off the critical path: the warp sleeps between polls.
-__device__ __forceinline__ bool mbar_wait_sleepy_abortable(uint64_t* bar, uint32_t parity, int code, int* abort) {
-  volatile int* ab = abort;
+__device__ __forceinline__ uint32_t clock32() {
+  uint32_t t;
+  asm volatile("mov.u32 %0, %%clock;" : "=r"(t));
+  return t;
+}
+
+// Whether a wait that began at `t0` ends without its barrier: the limit has run
+// out (reported, and `*abort` set), or `*abort` is set. A function of its own,
+// so that the many waits of a kernel stay a few instructions each.
+__device__ __noinline__ bool wait_gave_up(uint32_t t0, int code, int* abort) {
+  if (*reinterpret_cast<volatile int*>(abort)) return true;
+  if ((long long)(clock32() - t0) <= min(wait_limit(), kWaitCycles)) return false;  // (below the counter's wrap)
+  report(code);
+  *reinterpret_cast<volatile int*>(abort) = 1;
+  return true;
+}
+
+// mbar_wait_abortable in a compact form; `nap` > 0 sleeps that many nanoseconds
+// between polls, for a wait off the critical path.
+__device__ __forceinline__ bool mbar_wait_or_abort(uint64_t* bar, uint32_t parity, int code, int* abort, int nap) {
   if (mbar_try_wait(bar, parity)) return true;
-  const long long limit = wait_limit();
-  const long long t0 = clock64();
-  while (true) {
-    if (*ab) return false;
-    if (clock64() - t0 > limit) {
-      report(code);
-      *ab = 1;
-      return false;
-    }
-    __nanosleep(128);
-    if (mbar_try_wait(bar, parity)) return true;
-  }
+  const uint32_t t0 = clock32();
+  do {
+    if (wait_gave_up(t0, code, abort)) return false;
+    if (nap) __nanosleep(nap);
+  } while (!mbar_try_wait(bar, parity));
+  return true;
 }
 
 // This thread's shared-memory accesses so far come before the asynchronous
@@ -198,6 +222,12 @@ __device__ __forceinline__ void drain_ring(uint64_t* ring, int stages, int issue
   for (int i = issued > stages ? issued - stages : 0; i < issued; ++i)
     mbar_drain(&ring[i % stages], (uint32_t)(i / stages) & 1);
 }
+
+// Programmatic dependent launch: let the next kernel of the stream start its
+// prologue now, and wait in that prologue until the kernel before has completed
+// and its writes are visible (no effect in an ordinary launch).
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_prior_grid() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // ---------------------------------------------------------------- TMA
 // 2-D tiled tensor load into this CTA's shared memory, completion counted in

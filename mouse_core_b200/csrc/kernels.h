@@ -217,6 +217,7 @@ struct ChunkMetaParams {
 cudaError_t launch_chunk_meta(const ChunkMetaParams& p, cudaStream_t stream);
 
 struct ChunkEntry;
+struct ChunkSplit;
 struct ChunkParams {
   __nv_bfloat16* out;          // [tokens, Hq, HD]
   const int32_t* block_table;  // [batch, max_pages]
@@ -230,8 +231,8 @@ struct ChunkParams {
   float scale_log2;
   // the plan and the split tiles' partials (inside the caller's workspace)
   const ChunkEntry* entries;
+  const ChunkSplit* splits;
   int* head;
-  int* counters;
   float2* part_ml;
   float* part_o;
   int part_rows;
@@ -239,7 +240,7 @@ struct ChunkParams {
 struct ChunkLayout {
   size_t max_entries, max_slots;
   int part_rows;
-  size_t head, entries, counters, part_ml, part_o, total;
+  size_t head, entries, splits, part_ml, part_o, total;
 };
 int chunk_sub_tokens(int G);
 size_t chunk_layout(int batch, int tokens, int Hq, int Hkv, int head_dim, int sms, ChunkLayout* lay);
@@ -247,9 +248,10 @@ cudaError_t launch_chunk_plan(const ChunkParams& p, const ChunkLayout& lay, uint
                               cudaStream_t stream);
 // qm / sqm: 3-D token maps with boxes of a sub-tile's / a small tile's queries;
 // km / vm: the decode kernel's 64 x 64-box maps of one layer's K / V pool.
+// after_plan: the plan was launched just before on the same stream.
 cudaError_t launch_chunk_attention(const CUtensorMap& qm, const CUtensorMap& sqm, const CUtensorMap& km,
                                    const CUtensorMap& vm, ChunkParams p, const ChunkLayout& lay, uint8_t* ws, int sms,
-                                   cudaStream_t stream);
+                                   bool after_plan, cudaStream_t stream);
 
 // Token embedding (embed.cu).
 struct EmbedParams {

@@ -210,6 +210,20 @@ __device__ __forceinline__ void umma_ts_t128_linear_warp(uint32_t d, uint32_t a,
       ::"r"(d), "r"(a), "l"(db), "r"(idesc), "r"(accumulate));
 }
 
+// Half of umma_ts_t128_linear_warp: 64 tokens in four K-steps (the second half
+// is the same call with a + 32, db + 512 and accumulate = 1).
+__device__ __forceinline__ void umma_ts_t64_linear_warp(uint32_t d, uint32_t a, uint64_t db, uint32_t idesc,
+                                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred e, t, p;\n\t.reg .b32 ta;\n\t.reg .b64 b;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\tsetp.eq.b32 t, %3, %3;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "add.u32 ta, %1, 8;\n\tadd.s64 b, %2, 128;\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ta], b, %3, t;\n\t"
+      "add.u32 ta, %1, 16;\n\tadd.s64 b, %2, 256;\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ta], b, %3, t;\n\t"
+      "add.u32 ta, %1, 24;\n\tadd.s64 b, %2, 384;\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ta], b, %3, t;\n\t}"
+      ::"r"(d), "r"(a), "l"(db), "r"(idesc), "r"(accumulate));
+}
+
 __device__ __forceinline__ void umma_commit_warp(uint64_t* bar) {
   asm volatile(
       "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"

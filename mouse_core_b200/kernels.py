@@ -38,7 +38,7 @@ def _p(t):
 
 
 def _stream(t: torch.Tensor):
-    return torch.cuda.current_stream(t.device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def decode_workspace_bytes(batch: int, kv_heads: int, q_rows: int, head_dim: int, max_kv_len: int) -> int:
@@ -252,10 +252,14 @@ def decode_step_meta_launch(args: tuple, use_new_page: bool, stream: int) -> Non
     _count()
 
 
-def _same_device(ref: torch.Tensor, **tensors) -> None:
+def _check_on(dev: int, dtype, **tensors) -> None:
+    """Every tensor (``None`` is skipped) is contiguous, of ``dtype`` and on CUDA device ``dev``."""
     for name, t in tensors.items():
-        if t is not None and t.device != ref.device:
-            raise ValueError(f"{name} must be on {ref.device}, got {t.device}")
+        if t is None or (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == dev >= 0
+                         and t.is_contiguous()):
+            continue
+        _need(t, name, dtype)
+        raise ValueError(f"{name} must be on cuda:{dev}, got {t.device}")
 
 
 def chunk_meta(lengths: torch.Tensor, kv_len: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
@@ -277,21 +281,23 @@ def chunk_meta(lengths: torch.Tensor, kv_len: torch.Tensor, block_table: torch.T
     from ``free_pages``). A step that does not fit is reported through
     ``_lib.device_status`` (3: out of pages or table columns, 7: out of
     tokens) and its tokens without a page get slot -1."""
-    for name, t in (("lengths", lengths), ("kv_len", kv_len), ("block_table", block_table),
-                    ("free_pages", free_pages)):
-        _need(t, name, torch.int32)
+    _need(lengths, "lengths", torch.int32)
+    dev = lengths.get_device()
+    _check_on(dev, torch.int32, kv_len=kv_len, block_table=block_table, free_pages=free_pages)
     B, T = lengths.numel(), int(n_tokens)
     if lengths.ndim != 1 or kv_len.shape != lengths.shape or block_table.ndim != 2 or block_table.shape[0] != B:
         raise ValueError("lengths and kv_len must be [B] and block_table [B, max_pages]")
     if T < 0 or page_size <= 0:
         raise ValueError("n_tokens must be >= 0 and page_size > 0")
-    _same_device(lengths, kv_len=kv_len, block_table=block_table, free_pages=free_pages)
-    with torch.cuda.device(lengths.device):
-        buf = torch.empty(3 * B + 2 + 2 * T, dtype=torch.int32, device=lengths.device)
-        cu_q, cu_pages, new_len, q_pos, slot = buf.split((B + 1, B + 1, B, T, T))
-        _lib.call("mb_chunk_meta", _p(lengths), _p(kv_len), B, _p(block_table), block_table.shape[1], int(page_size),
-                  _p(free_pages), free_pages.numel(), T, _p(cu_q), _p(cu_pages), _p(new_len), _p(q_pos), _p(slot),
-                  _stream(lengths))
+    if torch.cuda.current_device() != dev:
+        with torch.cuda.device(dev):
+            return chunk_meta(lengths, kv_len, block_table, free_pages, page_size, n_tokens)
+    buf = torch.empty(3 * B + 2 + 2 * T, dtype=torch.int32, device=lengths.device)
+    cu_q, cu_pages, new_len, q_pos, slot = buf.split_with_sizes((B + 1, B + 1, B, T, T))
+    at = buf.data_ptr()
+    _lib.call("mb_chunk_meta", lengths.data_ptr(), kv_len.data_ptr(), B, block_table.data_ptr(), block_table.shape[1],
+              page_size, free_pages.data_ptr(), free_pages.numel(), T, at, at + 4 * (B + 1), at + 8 * (B + 1),
+              at + 4 * (3 * B + 2), at + 4 * (3 * B + 2 + T), _stream(lengths))
     _count()
     return cu_q, q_pos, slot, new_len, cu_pages
 
@@ -305,13 +311,13 @@ def chunk_plan(cu_q: torch.Tensor, kv_len: torch.Tensor, tokens: int, q_heads: i
                page_size: int, max_pages: int, workspace: torch.Tensor) -> None:
     """The work list of a ragged step, for ``chunk_attention(...,
     plan_ready=True)`` with the same sizes in every layer of the step."""
-    for name, t in (("cu_q", cu_q), ("kv_len", kv_len)):
-        _need(t, name, torch.int32)
-    _need(workspace, "workspace", torch.uint8)
+    _need(cu_q, "cu_q", torch.int32)
+    dev = cu_q.get_device()
+    _check_on(dev, torch.int32, kv_len=kv_len)
+    _check_on(dev, torch.uint8, workspace=workspace)
     if kv_len.ndim != 1 or cu_q.shape != (kv_len.numel() + 1,):
         raise ValueError("cu_q [B + 1] and kv_len [B] must match")
-    _same_device(cu_q, kv_len=kv_len, workspace=workspace)
-    with torch.cuda.device(cu_q.device):
+    with torch.cuda.device(dev):
         _lib.call("mb_chunk_plan", _p(cu_q), _p(kv_len), kv_len.numel(), int(tokens), q_heads, kv_heads, head_dim,
                   int(page_size), int(max_pages), _p(workspace), workspace.numel(), _stream(cu_q))
     _count()
@@ -331,39 +337,37 @@ def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     ``chunk_workspace_bytes``) is allocated for the call when not given;
     ``plan_ready`` takes the work list that ``chunk_plan`` left in it."""
     _need(q, "q", BF16, contiguous=False)
-    _need(k_pool, "k_pool", BF16)
-    _need(v_pool, "v_pool", BF16)
-    for name, t in (("block_table", block_table), ("cu_q", cu_q), ("kv_len", kv_len)):
-        _need(t, name, torch.int32)
+    dev = q.get_device()
+    _check_on(dev, BF16, k_pool=k_pool, v_pool=v_pool, out=out)
+    _check_on(dev, torch.int32, block_table=block_table, cu_q=cu_q, kv_len=kv_len)
     if q.ndim != 3 or k_pool.ndim != 4 or k_pool.shape != v_pool.shape:
         raise ValueError("q must be [T, Hq, hd] and the pools [P, Hkv, page, hd] of equal shape")
     T, Hq, hd = q.shape
     P, Hkv, page, hd2 = k_pool.shape
     if hd2 != hd:
         raise ValueError(f"head_dim mismatch: q {hd}, pool {hd2}")
-    if q.stride(2) != 1 or (Hq > 1 and q.stride(1) != hd):
+    stride, head_stride, unit = q.stride()
+    if unit != 1 or (Hq > 1 and head_stride != hd):
         raise ValueError("q's heads must be contiguous")
     B = kv_len.numel()
     if kv_len.ndim != 1 or cu_q.shape != (B + 1,) or block_table.ndim != 2 or block_table.shape[0] != B:
         raise ValueError("block_table [B, max_pages], cu_q [B + 1] and kv_len [B] must match")
-    if out is not None:
-        _need(out, "out", BF16)
-        if out.shape != q.shape:
-            raise ValueError("out must have q's shape")
+    if out is not None and out.shape != q.shape:
+        raise ValueError("out must have q's shape")
     if workspace is not None:
-        _need(workspace, "workspace", torch.uint8)
+        _check_on(dev, torch.uint8, workspace=workspace)
     elif plan_ready:
         raise ValueError("plan_ready needs the workspace that holds the plan")
-    _same_device(q, k_pool=k_pool, v_pool=v_pool, block_table=block_table, cu_q=cu_q, kv_len=kv_len, out=out,
-                 workspace=workspace)
-    with torch.cuda.device(q.device):
-        if out is None:
-            out = torch.empty(T, Hq, hd, dtype=BF16, device=q.device)
-        if workspace is None:
-            workspace = torch.empty(chunk_workspace_bytes(B, T, Hq, Hkv, hd), dtype=torch.uint8, device=q.device)
-        _lib.call("mb_chunk_attention", _p(q), q.stride(0) if T > 1 else Hq * hd, _p(k_pool), _p(v_pool), P,
-                  _p(block_table), block_table.shape[1], _p(cu_q), _p(kv_len), B, T, Hq, Hkv, hd, page, float(scale),
-                  int(plan_ready), _p(out), _p(workspace), workspace.numel(), _stream(q))
+    if torch.cuda.current_device() != dev:
+        with torch.cuda.device(dev):
+            return chunk_attention(q, k_pool, v_pool, block_table, cu_q, kv_len, scale, out, workspace, plan_ready)
+    if out is None:
+        out = torch.empty((T, Hq, hd), dtype=BF16, device=q.device)
+    if workspace is None:
+        workspace = torch.empty(chunk_workspace_bytes(B, T, Hq, Hkv, hd), dtype=torch.uint8, device=q.device)
+    _lib.call("mb_chunk_attention", q.data_ptr(), stride if T > 1 else Hq * hd, k_pool.data_ptr(), v_pool.data_ptr(), P,
+              block_table.data_ptr(), block_table.shape[1], cu_q.data_ptr(), kv_len.data_ptr(), B, T, Hq, Hkv, hd, page,
+              scale, plan_ready, out.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream(q))
     _count(1 if plan_ready else 2)
     return out
 
