@@ -11,7 +11,9 @@
 // Work. The G q-heads of a kv-head read the same keys, so their queries share
 // tiles: query row r of a tile is (token r / G, head r % G). A row with
 // n_b G <= 16 is one "small" tile; a longer one is cut into "big" tiles of two
-// sub-tiles of TS = 128 / G tokens (128 query rows) each. Every (tile,
+// sub-tiles of TS = 128 / G tokens (128 query rows) each. (A big tile with one
+// sub-tile's tokens takes its even key tiles as the one and its odd ones as the
+// other, "dual", and the epilogue joins the two.) Every (tile,
 // kv-head) is one item over 128-key tiles of the cache; items with many key
 // tiles are split along the keys into pieces when the step has too few items
 // to fill the SMs (chunk_plan_kernel): each piece leaves (O, max, sum) in fp32,
@@ -75,10 +77,17 @@ constexpr int kMinSplitTiles = 4;
 // the step: longest first already evens those out.
 constexpr int kPiecesPerShare = 3;
 
+// What a key tile costs, in units of half a tile of a small piece or of one with
+// a single sub-tile (both bound by the K/V they read): two sub-tiles' softmax
+// takes 1.3 times that at head_dim 128 (64 KB of K/V a tile) and twice at 64.
+__host__ __device__ constexpr int chunk_tile_cost(bool two_subs, int head_dim) {
+  return !two_subs ? 2 : head_dim == 128 ? 3 : 4;
+}
+
 struct ChunkPlanParams {
   const int32_t* cu_q;
   const int32_t* kv_len;
-  int batch, tokens, G, Hkv, tile_tokens, key_limit, sms, max_entries, max_slots;
+  int batch, tokens, G, Hkv, tile_tokens, key_limit, sms, max_entries, max_slots, two_subs_cost;
   ChunkEntry* entries;
   ChunkSplit* splits;
   int* head;  // [0] entries, [1] next item, [2] CTAs done, [3] splits
@@ -91,8 +100,8 @@ __device__ __forceinline__ int chunk_key_tiles(int n, int len, int t, bool small
 }
 
 // The work list of a step, in one block with a row per thread. Splitting: with
-// E entries before it, the longest tiles are cut into pieces of at most c key
-// tiles, c the smallest that leaves at most one wave of CTAs beyond the waves
+// E entries before it, the longest tiles are cut into pieces that cost at most
+// c, c the smallest that leaves at most one wave of CTAs beyond the waves
 // the unsplit items need anyway (so the partials stay few), and not below the
 // two bounds above. Order: rows by the length of their longest piece, longest
 // first; a row's tiles stay together, its last (longest) first, so that they
@@ -111,6 +120,7 @@ __global__ void __launch_bounds__(kChunkPlanThreads) chunk_plan_kernel(const Chu
   // Row r0 + tid: its tokens, keys and tiles.
   int r0 = -1, n = 0, len = 0, tiles = 0, cu = 0;
   bool small = false;
+  int cost = 2;  // of a key tile
   auto load = [&](int at) {
     if (at == r0) return;
     r0 = at;
@@ -121,6 +131,7 @@ __global__ void __launch_bounds__(kChunkPlanThreads) chunk_plan_kernel(const Chu
       len = max(p.kv_len[r0 + tid], 0);
       small = n <= kChunkSmallRows / p.G;
       tiles = n <= 0 ? 0 : small ? 1 : (n + p.tile_tokens - 1) / p.tile_tokens;
+      cost = n > p.tile_tokens / 2 ? p.two_subs_cost : 2;
     }
   };
   auto key_tiles = [&](int t) { return chunk_key_tiles(n, len, t, small, p.tile_tokens, p.key_limit); };
@@ -130,7 +141,7 @@ __global__ void __launch_bounds__(kChunkPlanThreads) chunk_plan_kernel(const Chu
     return v;
   };
 
-  // 1. Entries, key tiles and the most of one entry, over all rows.
+  // 1. Entries, their cost and the most of one, over all rows.
   if (tid < 3) fit_s[tid] = 0;
   if (tid == 0) slots_s = splits_s = 0;
   hist[tid] = 0;
@@ -141,8 +152,8 @@ __global__ void __launch_bounds__(kChunkPlanThreads) chunk_plan_kernel(const Chu
     load(at);
     if (n > 0 && len > p.key_limit) report(kDevBadPage);
     count += tiles;
-    for (int t = 0; t < tiles; ++t) sum += key_tiles(t);
-    if (tiles > 0) most = max(most, key_tiles(tiles - 1));
+    for (int t = 0; t < tiles; ++t) sum += key_tiles(t) * cost;
+    if (tiles > 0) most = max(most, key_tiles(tiles - 1) * cost);
   }
   count = warp_add(count);
   sum = warp_add(sum);
@@ -164,14 +175,14 @@ __global__ void __launch_bounds__(kChunkPlanThreads) chunk_plan_kernel(const Chu
   if (room > E) {
     const unsigned long long share = sum * p.Hkv / (kPiecesPerShare * p.sms);
     lo = (int)min((unsigned long long)hi, max(max((sum + room - 1) / (unsigned long long)room, share),
-                                              (unsigned long long)kMinSplitTiles));
+                                              (unsigned long long)(2 * kMinSplitTiles)));
   }
   for (int round = 0; lo < hi; ++round) {
     const int c = (lo + hi) >> 1;
     unsigned long long pieces = 0;
     for (int at = 0; at < p.batch; at += blockDim.x) {
       load(at);
-      for (int t = 0; t < tiles; ++t) pieces += (key_tiles(t) + c - 1) / c;
+      for (int t = 0; t < tiles; ++t) pieces += (key_tiles(t) * cost + c - 1) / c;
     }
     pieces = warp_add(pieces);
     if (lane == 0 && pieces) atomicAdd(&fit_s[round % 3], pieces);
@@ -183,16 +194,16 @@ __global__ void __launch_bounds__(kChunkPlanThreads) chunk_plan_kernel(const Chu
       lo = c + 1;
   }
   const int c = hi;
-  auto pieces_of = [&](int kt) { return kt <= c ? 1 : (kt + c - 1) / c; };
+  auto pieces_of = [&](int of) { return of <= c ? 1 : (of + c - 1) / c; };  // of a tile, by its cost
   auto row_pieces = [&]() {
-    if (tiles == 0 || key_tiles(tiles - 1) <= c) return tiles;
+    if (tiles == 0 || key_tiles(tiles - 1) * cost <= c) return tiles;
     int s = 0;
-    for (int t = 0; t < tiles; ++t) s += pieces_of(key_tiles(t));
+    for (int t = 0; t < tiles; ++t) s += pieces_of(key_tiles(t) * cost);
     return s;
   };
   // Of the row's longest piece (a row with a split tile counts as c: it has
   // pieces near it); 0 comes first.
-  auto bucket = [&]() { return kBuckets - 1 - min(min(key_tiles(tiles - 1), c), kBuckets - 1); };
+  auto bucket = [&]() { return kBuckets - 1 - min(min(key_tiles(tiles - 1) * cost, c) / 2, kBuckets - 1); };
   // 3. Where each piece length starts in the order.
   __syncthreads();
   for (int at = 0; at < p.batch; at += blockDim.x) {
@@ -261,12 +272,13 @@ __global__ void __launch_bounds__(kChunkPlanThreads) chunk_plan_kernel(const Chu
       const int n_ = n_s[r], len_ = len_s[r];
       const bool small_ = n_ <= kChunkSmallRows / p.G;
       const int kt = chunk_key_tiles(n_, len_, t, small_, p.tile_tokens, p.key_limit);
-      const int pieces = pieces_of(kt);
+      const int cost_ = n_ > p.tile_tokens / 2 ? p.two_subs_cost : 2;
+      const int pieces = pieces_of(kt * cost_);
       // Behind the row's longer tiles t + 1 .. last.
       int first = base_s[r] + last - t;
-      if (chunk_key_tiles(n_, len_, last, small_, p.tile_tokens, p.key_limit) > c)
+      if (chunk_key_tiles(n_, len_, last, small_, p.tile_tokens, p.key_limit) * cost_ > c)
         for (int u = t + 1; u <= last; ++u)
-          first += pieces_of(chunk_key_tiles(n_, len_, u, small_, p.tile_tokens, p.key_limit)) - 1;
+          first += pieces_of(chunk_key_tiles(n_, len_, u, small_, p.tile_tokens, p.key_limit) * cost_) - 1;
       int slot = -1;
       if (pieces > 1) {
         slot = atomicAdd(&slots_s, pieces);
@@ -318,24 +330,26 @@ struct ChunkTile {
   // for P beside S, so that the next S = Q K^T runs under a tile's exponentials;
   // with 128 P overwrites its S.
   static constexpr bool OWN_P = HD == 64;
+  static constexpr int FMA_EXP = HD == 128 ? 3 : 99;  // pairs of exponentials on the FMA pipe: those whose index has these low bits set
   static constexpr uint32_t T_O = 256, T_P = OWN_P ? 384 : 0, P_STEP = OWN_P ? 64 : 128;
 };
 
 constexpr int kChunkMaxStages = 5;
 // A piece as its CTA's warps see it.
 struct ChunkWork {
-  int h;             // kv-head, or -1: no work left
+  int h, row;        // kv-head, or -1: no work left; the step's row
   int q0, ntok, pos0;
   int len;           // keys the row holds
   int k0, n;         // key tiles of the piece
   int n0, n1;        // ... that sub-tile 0 and 1 visit (big)
-  int slot, pieces, piece, small;
+  int slot, pieces, piece, small, dual;
 };
 
 struct ChunkShared {
   uint64_t work_full[2], work_empty[2];   // descriptor ring (producer -> everyone)
   uint64_t q_full[2][2], q_empty[2][2];   // by piece parity and sub-tile; q_empty: its Q, or the join area, is free
-  uint64_t k_full[kChunkMaxStages], v_full[kChunkMaxStages], kv_empty[kChunkMaxStages];
+  uint64_t k_full[kChunkMaxStages], v_full[kChunkMaxStages];
+  uint64_t k_empty[kChunkMaxStages], v_empty[kChunkMaxStages];
   uint64_t v_tail[kChunkMaxStages];       // a V tile with rows behind the last token has landed (by such tile)
   uint64_t small_done[kChunkMaxStages];   // a small tile's keys are consumed (by small tile)
   uint64_t s_full[2], p_full[2][2];       // per sub-tile; P in two halves of 64 keys
@@ -347,9 +361,16 @@ struct ChunkShared {
   int abort;                              // set by the first wait that runs out
   int q_armed[2];                         // pieces whose Q loads were issued
   ChunkWork work[2];
+  alignas(16) int box_y[32];              // the pool rows of the next 16 tiles' boxes
   float stats[2][2][2][128];              // [piece parity][sub-tile][max, sum][row]; small: [.][0][.][warp * 16 + row]
 };
 static_assert(sizeof(ChunkShared) <= ChunkTile<128>::BARS, "barrier block outgrew its share");
+
+// A number known at compile time.
+template <int V>
+struct Const {
+  __device__ constexpr operator int() const { return V; }
+};
 
 // A position in a ring of N barriers and the parity of its phase.
 template <int N>
@@ -404,7 +425,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(&sh->k_full[s], 1);
       mbar_init(&sh->v_full[s], 1);
-      mbar_init(&sh->kv_empty[s], 1);
+      mbar_init(&sh->k_empty[s], 1);
+      mbar_init(&sh->v_empty[s], 1);
       mbar_init(&sh->v_tail[s], 1);
       mbar_init(&sh->small_done[s], 8);
     }
@@ -423,12 +445,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 
   // Warp-uniform bounded wait; one that runs out stops every warp of the CTA.
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
-    return (bool)__all_sync(0xffffffffu, mbar_wait_or_abort(bar, parity, code, &sh->abort, 0));
+    return (bool)__all_sync(0xffffffffu, mbar_wait_or_abort(bar, parity, code, &sh->abort));
   };
   // The same off the critical path: it sleeps between polls and so leaves the
   // issue slots to the warps at work.
   auto sleepy = [&](uint64_t* bar, uint32_t parity) {
-    return (bool)__all_sync(0xffffffffu, mbar_wait_or_abort(bar, parity, kDevTimeoutFull, &sh->abort, 128));
+    return (bool)__all_sync(0xffffffffu, mbar_wait_sleepy_or_abort(bar, parity, kDevTimeoutFull, &sh->abort));
   };
   // Piece k of this CTA from the descriptor ring (h < 0: the end of the work);
   // take() is false at the end, too.
@@ -448,61 +470,29 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   if (warp < 4) {
     if (warp == 0) {
       // ---------------------------------------------------------- producer
+      // Lane 0 waits and loads; the warp looks the boxes' pages up.
       if (lane == 0) {
         prefetch_tensormap(&qmap);
         prefetch_tensormap(&sqmap);
         prefetch_tensormap(&kmap);
         prefetch_tensormap(&vmap);
       }
+      auto wait1 = [&](uint64_t* bar, uint32_t parity) {
+        return mbar_wait_or_abort(bar, parity, kDevTimeoutEmpty, &sh->abort);
+      };
       const int n_items = p.head[0] * p.Hkv;
       // The next piece is taken, and its entry read, when this one's last tiles
       // are loaded: early enough to hide the reads, late enough that a CTA
       // busy with a long piece does not hold on to another.
-      int next = 0;
+      int next = blockIdx.x;
       ChunkEntry e{};
-      auto fetch = [&](int k) {
-        if (lane == 0) next = k == 0 ? (int)blockIdx.x : (int)gridDim.x + atomicAdd(&p.head[1], 1);
-        next = __shfl_sync(0xffffffffu, next, 0);
-        if (next < n_items) e = p.entries[next / p.Hkv];
-      };
-      fetch(0);
-      bool ok = true;
+      if (next < n_items) e = p.entries[next / p.Hkv];
       Ring kv, tail_at;
-      int issued = 0, tails_issued = 0;  // K/V tiles, and those with V rows to be zeroed
-      uint32_t tails = 0;                // bit i: the tile issued i tiles ago was one of them
+      int k_issued = 0, issued = 0, tails_issued = 0;  // K tiles, V tiles, and those with V rows to be zeroed
+      uint32_t tails = 0;                              // bit i: the tile issued i tiles ago was one of them
       for (int k = 0;; ++k) {
-        if (!(ok = wait(&sh->work_empty[k & 1], ((k >> 1) & 1) ^ 1, kDevTimeoutEmpty))) break;
-        if (next >= n_items) {
-          if (lane == 0) {
-            sh->work[k & 1].h = -1;
-            mbar_arrive(&sh->work_full[k & 1]);
-          }
-          break;
-        }
+        bool ok = true;
         ChunkWork wk;
-        wk.h = next % p.Hkv;
-        const int row = e.a.x;
-        wk.q0 = e.a.y;
-        wk.ntok = e.a.z;
-        wk.pos0 = e.a.w;
-        wk.len = e.b.x;
-        wk.k0 = e.b.y;
-        wk.n = e.b.z;
-        wk.slot = e.b.w;
-        wk.pieces = e.c.x;
-        wk.piece = e.c.y;
-        wk.small = e.c.z;
-        wk.n0 = wk.n;
-        wk.n1 = 0;
-        if (wk.ntok > p.sub_tokens && !wk.small) {
-          const int keys0 = min(wk.pos0 + p.sub_tokens, p.key_limit);
-          wk.n0 = min(max(max(1, (max(keys0, 0) + kChunkKeys - 1) / kChunkKeys) - wk.k0, 0), wk.n);
-          wk.n1 = wk.n;
-        }
-        if (lane == 0) {
-          sh->work[k & 1] = wk;
-          mbar_arrive(&sh->work_full[k & 1]);
-        }
         // Q: the small buffer of this parity is free once piece k - 2 is done, a
         // sub-tile's (the small pieces' join area) once piece k - 1 is. The
         // second sub-tile's is loaded behind the first K/V tile, whose stage is
@@ -510,81 +500,130 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         auto load_q = [&](int s) {
           const int par = wk.small ? k & 1 : (k - 1) & 1;
           const uint32_t phase = wk.small ? ((k >> 1) & 1) ^ 1 : ((k - 1) >> 1) & 1;
-          if (k >= (wk.small ? 2 : 1) && !wait(&sh->q_empty[par][s], phase, kDevTimeoutEmpty)) return false;
-          if (wk.small && k >= 2 && !wait(&sh->q_empty[par][1], phase, kDevTimeoutEmpty)) return false;
-          if (lane == 0) {
-            uint64_t* bar = &sh->q_full[k & 1][s];
-            mbar_arrive_expect_tx(bar, C::NCB * (wk.small ? p.small_rows : p.sub_tokens * p.G) * 128);
+          if (k >= (wk.small ? 2 : 1) && !wait1(&sh->q_empty[par][s], phase)) return false;
+          if (wk.small && k >= 2 && !wait1(&sh->q_empty[par][1], phase)) return false;
+          uint64_t* bar = &sh->q_full[k & 1][s];
+          mbar_arrive_expect_tx(bar, C::NCB * (wk.small ? p.small_rows : p.sub_tokens * p.G) * 128);
+          uint8_t* dst = wk.small ? sq + (k & 1) * C::SQ : qs + s * C::QTILE;
+          const CUtensorMap* map = wk.small ? &sqmap : &qmap;
 #pragma unroll
-            for (int cb = 0; cb < C::NCB; ++cb) {
-              uint8_t* dst = wk.small ? sq + (k & 1) * C::SQ + cb * C::SQBOX : qs + s * C::QTILE + cb * C::BOX;
-              tma_load_3d(dst, wk.small ? &sqmap : &qmap, bar, cb * 64, wk.h * p.G, wk.q0 + s * p.sub_tokens);
-            }
-            *reinterpret_cast<volatile int*>(&sh->q_armed[s]) = k + 1;
-          }
+          for (int cb = 0; cb < C::NCB; ++cb, dst += wk.small ? C::SQBOX : C::BOX)
+            tma_load_3d(dst, map, bar, cb * 64, wk.h * p.G, wk.q0 + s * p.sub_tokens);
+          *reinterpret_cast<volatile int*>(&sh->q_armed[s]) = k + 1;
           return true;
         };
-        if (!(ok = load_q(0))) break;
-        if (wk.n1 == 0 && lane == 0) {  // nothing to load: both advance with every piece
-          mbar_arrive(&sh->q_full[k & 1][1]);
-          *reinterpret_cast<volatile int*>(&sh->q_armed[1]) = k + 1;
-        }
-        // K/V tiles. Page ids of the next 32 boxes at a time, one per lane.
-        const int32_t* table = p.block_table + (size_t)row * p.max_pages;
-        int y_lane = 0;
-        for (int j = 0; j < wk.n; ++j) {
-          if (j % 16 == 0) {
-            const long long tok = ((long long)wk.k0 + j) * kChunkKeys + lane * 64;
-            y_lane = -64;  // wholly out of bounds: reads zeros
-            if (tok < wk.len && tok < ((long long)wk.k0 + wk.n) * kChunkKeys) {
-              const int col = (int)tok / p.page_size;
-              const int pg = col < p.max_pages ? table[col] : -1;
-              if (pg >= 0 && pg < p.num_pages)
-                y_lane = (pg * p.Hkv + wk.h) * p.page_size + (int)tok % p.page_size;
-              else
-                report(kDevBadPage);
-            }
+        if (lane == 0) {
+          wk.h = next < n_items ? next % p.Hkv : -1;
+          wk.row = e.a.x;
+          wk.q0 = e.a.y;
+          wk.ntok = e.a.z;
+          wk.pos0 = e.a.w;
+          wk.len = e.b.x;
+          wk.k0 = e.b.y;
+          wk.n = e.b.z;
+          wk.slot = e.b.w;
+          wk.pieces = e.c.x;
+          wk.piece = e.c.y;
+          wk.small = e.c.z;
+          wk.n0 = wk.n;
+          wk.n1 = 0;
+          if (wk.ntok > p.sub_tokens && !wk.small) {
+            const int keys0 = min(wk.pos0 + p.sub_tokens, p.key_limit);
+            wk.n0 = min(max(max(1, (max(keys0, 0) + kChunkKeys - 1) / kChunkKeys) - wk.k0, 0), wk.n);
+            wk.n1 = wk.n;
           }
-          if (j == max(wk.n - 2, 0)) fetch(k + 1);
-          const int y0 = __shfl_sync(0xffffffffu, y_lane, 2 * (j % 16));
-          const int y1 = __shfl_sync(0xffffffffu, y_lane, 2 * (j % 16) + 1);
-          if (!(ok = wait(&sh->kv_empty[kv.at], kv.phase ^ 1, kDevTimeoutEmpty))) break;
-          const bool tail = ragged(wk.k0 + j, wk.len);
-          if (lane == 0) {
-            uint64_t* bar = &sh->k_full[kv.at];
-            const CUtensorMap* map = &kmap;
-            uint8_t* dst = ks + kv.at * C::KVTILE;
-#pragma unroll 1
-            for (int i = 0; i < 2; ++i) {
-              mbar_arrive_expect_tx(bar, C::KVTILE);
-#pragma unroll
-              for (int cb = 0; cb < C::NCB; ++cb) {
-                tma_load_2d(dst + cb * C::BOX, map, bar, cb * 64, y0);
-                tma_load_2d(dst + cb * C::BOX + C::BOX / 2, map, bar, cb * 64, y1);
+          wk.dual = !wk.small && wk.ntok <= p.sub_tokens && wk.n > 1;
+          if (wk.dual) {
+            wk.n0 = (wk.n + 1) / 2;
+            wk.n1 = wk.n / 2;
+          }
+          ok = wait1(&sh->work_empty[k & 1], ((k >> 1) & 1) ^ 1);
+          if (ok) {
+            sh->work[k & 1] = wk;
+            mbar_arrive(&sh->work_full[k & 1]);
+          } else {
+            wk.h = -1;
+          }
+        }
+        const int h = __shfl_sync(0xffffffffu, wk.h, 0);
+        if (h < 0) break;
+        // K/V tiles in 64-row boxes, the pages of 16 tiles' boxes looked up at a
+        // time (one per lane, while the 16 before are loaded). A box behind the
+        // row's last key, or on no page, reads zeros (wholly out of bounds).
+        const int n = __shfl_sync(0xffffffffu, wk.n, 0), k0 = __shfl_sync(0xffffffffu, wk.k0, 0);
+        const int len = __shfl_sync(0xffffffffu, wk.len, 0), row = __shfl_sync(0xffffffffu, wk.row, 0);
+        const int32_t* table = p.block_table + (size_t)row * p.max_pages;
+        int page = -1, at = 0;
+        auto look_up = [&](int j) {
+          const long long tok = ((long long)k0 + j) * kChunkKeys + lane * 64;
+          page = -2;  // behind the last key
+          if (tok < len && tok < ((long long)k0 + n) * kChunkKeys) {
+            const int col = (int)tok / p.page_size;
+            at = (int)tok - col * p.page_size;
+            page = col < p.max_pages ? table[col] : -1;
+          }
+        };
+        look_up(0);
+        if (lane == 0) {
+          ok = load_q(0);
+          if (ok && (wk.n1 == 0 || wk.dual)) {  // nothing to load: both advance with every piece
+            mbar_arrive(&sh->q_full[k & 1][1]);
+            *reinterpret_cast<volatile int*>(&sh->q_armed[1]) = k + 1;
+          }
+        }
+        for (int j0 = 0; j0 < n; j0 += 16) {
+          int y = -64;
+          if (page >= 0 && page < p.num_pages)
+            y = (page * p.Hkv + h) * p.page_size + at;
+          else if (page != -2)
+            report(kDevBadPage);
+          sh->box_y[lane] = y;
+          __syncwarp();
+          if (j0 + 16 < n) look_up(j0 + 16);
+          if (lane == 0 && ok) {
+            for (int j = j0; j < min(n, j0 + 16); ++j) {
+              if (j == max(n - 2, 0)) {
+                next = (int)gridDim.x + atomicAdd(&p.head[1], 1);
+                if (next < n_items) e = p.entries[next / p.Hkv];
               }
-              bar = tail ? &sh->v_tail[tail_at.at] : &sh->v_full[kv.at];
-              map = &vmap;
-              dst = vs + kv.at * C::KVTILE;
+              const int2 ys = *reinterpret_cast<const int2*>(&sh->box_y[2 * (j - j0)]);
+              // K and V stages are released apart: K's a tile earlier than V's.
+              const bool tail = ragged(k0 + j, len);
+              auto load = [&](uint64_t* bar, uint64_t* empty, const CUtensorMap* map, uint8_t* dst) {
+                if (!wait1(empty, kv.phase ^ 1)) return false;
+                mbar_arrive_expect_tx(bar, C::KVTILE);
+#pragma unroll
+                for (int cb = 0; cb < C::NCB; ++cb) {
+                  tma_load_2d(dst + cb * C::BOX, map, bar, cb * 64, ys.x);
+                  tma_load_2d(dst + cb * C::BOX + C::BOX / 2, map, bar, cb * 64, ys.y);
+                }
+                return true;
+              };
+              if (!(ok = load(&sh->k_full[kv.at], &sh->k_empty[kv.at], &kmap, ks + kv.at * C::KVTILE))) break;
+              ++k_issued;
+              if (!(ok = load(tail ? &sh->v_tail[tail_at.at] : &sh->v_full[kv.at], &sh->v_empty[kv.at], &vmap,
+                              vs + kv.at * C::KVTILE)))
+                break;
+              kv.step();
+              ++issued;
+              if (tail) {
+                tail_at.step();
+                ++tails_issued;
+              }
+              tails = tails << 1 | (uint32_t)tail;
+              if (j == 0 && wk.n1 > 0 && !wk.dual && !(ok = load_q(1))) break;
             }
           }
           __syncwarp();
-          kv.step();
-          ++issued;
-          if (tail) {
-            tail_at.step();
-            ++tails_issued;
-          }
-          tails = tails << 1 | (uint32_t)tail;
-          if (j == 0 && wk.n1 > 0 && !(ok = load_q(1))) break;
         }
-        if (!ok) break;
+        if (!__shfl_sync(0xffffffffu, ok, 0)) break;
       }
       if (lane == 0) {
         // Every load issued lands before the CTA exits, also when a wait ran out.
         for (int s = 0; s < 2; ++s)
           for (int n = *reinterpret_cast<volatile int*>(&sh->q_armed[s]), i = max(n - 2, 0); i < n; ++i)
             mbar_drain(&sh->q_full[i & 1][s], (uint32_t)(i >> 1) & 1);
-        drain_ring(sh->k_full, C::STAGES, issued);
+        drain_ring(sh->k_full, C::STAGES, k_issued);
         drain_ring(sh->v_tail, C::STAGES, tails_issued);
         for (int i = max(issued - C::STAGES, 0); i < issued; ++i)
           if (!(tails >> (issued - 1 - i) & 1)) mbar_drain(&sh->v_full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1);
@@ -596,9 +635,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       // --------------------------------------------------------- MMA issue
       constexpr uint32_t ID_QK = umma_idesc_bf16(128, 128, 0, 0);
       constexpr uint32_t ID_PV = umma_idesc_bf16(128, HD, 0, 1);
-      auto issue_qk = [&](int s, int st) {
+      auto issue_qk = [&](int s, int st, int q = -1) {
         tc_fence_after();
-        const uint64_t dq = umma_desc_sw128(smem_u32(qs + s * C::QTILE), 16, 1024);
+        const uint64_t dq = umma_desc_sw128(smem_u32(qs + (q < 0 ? s : q) * C::QTILE), 16, 1024);
         const uint64_t dk = umma_desc_sw128(smem_u32(ks + st * C::KVTILE), 16, 1024);
         if constexpr (HD == 128)
           umma_ss_k128_warp(tbase + 128 * s, dq, dk, ID_QK);
@@ -615,50 +654,72 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         if (wk.small) {
           for (int j = 0; j < wk.n; ++j, kv.step(), small_at.step()) {
             if (!(ok = wait(&sh->small_done[small_at.at], small_at.phase, kDevTimeoutFull))) break;
-            if (lane == 0) mbar_arrive(&sh->kv_empty[kv.at]);
+            if (lane == 0) {
+              mbar_arrive(&sh->k_empty[kv.at]);
+              mbar_arrive(&sh->v_empty[kv.at]);
+            }
           }
           ok = ok && take(++k, wk);
           continue;
         }
+        Ring kv1 = kv;  // the stage behind kv
+        kv1.step();
 #pragma unroll 1
         for (int s = early ? 1 : 0; s < 2; ++s) {
-          const int n_s = s == 0 ? wk.n0 : wk.n1;
+          const int n_s = s == 0 ? wk.n0 : wk.n1, q = wk.dual ? 0 : s;
           // (Q is waited for even when this piece has no key for the sub-tile: it must have landed.)
           if (!(ok = wait(&sh->q_full[k & 1][s], (k >> 1) & 1, kDevTimeoutFull))) break;
+          const Ring& first = wk.dual && s == 1 ? kv1 : kv;
           if (n_s > 0) {
-            if (!(ok = wait(&sh->k_full[kv.at], kv.phase, kDevTimeoutFull))) break;
-            issue_qk(s, kv.at);
+            if (!(ok = wait(&sh->k_full[first.at], first.phase, kDevTimeoutFull))) break;
+            issue_qk(s, first.at, q);
           }
-          if (n_s <= 1) umma_commit_warp(&sh->q_empty[k & 1][s]);  // its last Q K^T
+          if (wk.dual || s == 1) umma_commit_warp(&sh->k_empty[first.at]);
+          if (!wk.dual && n_s <= 1) umma_commit_warp(&sh->q_empty[k & 1][s]);  // its last Q K^T
+        }
+        if (ok && wk.dual && wk.n <= 2) {
+          umma_commit_warp(&sh->q_empty[k & 1][0]);
+          umma_commit_warp(&sh->q_empty[k & 1][1]);
         }
         if (!ok) break;
         early = false;
         ChunkWork nx;
         nx.h = -1;
         for (int j = 0; j < wk.n; ++j) {
-          Ring kv1 = kv;
+          kv1 = kv;  // the stage of the next S of the sub-tiles: one tile on, dual two
           kv1.step();
+          if (wk.dual) kv1.step();
+          const int ahead = wk.dual ? 2 : 1;
+          if (!(ok = wait(&sh->v_full[kv.at], kv.phase, kDevTimeoutFull))) break;
+          if (!wk.dual && j + 1 < wk.n && !(ok = wait(&sh->k_full[kv1.at], kv1.phase, kDevTimeoutFull))) break;
           const uint64_t dv = umma_desc_sw128(smem_u32(vs + kv.at * C::KVTILE), C::BOX, 1024);
-#pragma unroll 1
-          for (int s = 0; s < 2; ++s) {
-            const int n_s = s == 0 ? wk.n0 : wk.n1;
-            if (j >= n_s) continue;
+          // One sub-tile's step: O += P V for tile j and S = Q K^T for its next one.
+          // (At head_dim 128 written out for each: the tensor pipe idles while
+          // this warp works its way from one MMA to the next. At 64 the softmax is
+          // the bound, and the shorter code is worth more.)
+          auto step = [&](auto sub_tile) {
+            const int s = sub_tile;
+            const int n_s = wk.dual ? wk.n : s == 0 ? wk.n0 : wk.n1;
+            if (j >= n_s || (wk.dual && (j & 1) != s)) return true;
             const uint32_t par = tile_par >> s & 1;
             auto next_s = [&]() {
-              if (j + 1 >= n_s) return true;
-              if (!wait(&sh->k_full[kv1.at], kv1.phase, kDevTimeoutFull)) return false;
-              issue_qk(s, kv1.at);
-              if (j + 2 == n_s) umma_commit_warp(&sh->q_empty[k & 1][s]);
+              if (wk.dual && !wait(&sh->k_full[kv1.at], kv1.phase, kDevTimeoutFull)) return false;
+              issue_qk(s, kv1.at, wk.dual ? 0 : (int)s);
+              if (j + ahead + 1 == n_s) {
+                umma_commit_warp(&sh->q_empty[k & 1][s]);
+                if (wk.dual) umma_commit_warp(&sh->q_empty[k & 1][s ^ 1]);
+              }
               return true;
             };
-            if (C::OWN_P && j + 1 < n_s)  // S is free once it is in registers
-              if (!(ok = wait(&sh->s_read[s], par, kDevTimeoutFull) && next_s())) break;
-            if (s == 1 && j + 1 == wk.n) {
+            if (C::OWN_P && j + ahead < n_s) {  // S is free once it is in registers
+              if (!wait(&sh->s_read[s], par, kDevTimeoutFull) || !next_s()) return false;
+            }
+            if (s == 1 && j + 1 == wk.n && !wk.dual) {
               // While sub-tile 1 finishes the piece, sub-tile 0 starts the next
               // one as soon as its Q and K are there, so that the two stay out
               // of step (in step, their exponentials compete for the same unit).
-              if (!(ok = take_any(k + 1, nx))) break;
-              const bool cand = nx.h >= 0 && !nx.small && nx.n0 > 0;
+              if (!take_any(k + 1, nx)) return false;
+              const bool cand = nx.h >= 0 && !nx.small && !nx.dual && nx.n0 > 0;
               const uint32_t t0 = clock32();
               while (true) {
                 if (cand && !early &&
@@ -669,34 +730,43 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                   early = true;
                 }
                 if (__all_sync(0xffffffffu, mbar_test_wait(&sh->p_full[1][0], par))) break;
-                if (!(ok = __all_sync(0xffffffffu, !wait_gave_up(t0, kDevTimeoutFull, &sh->abort)))) break;
+                if (__any_sync(0xffffffffu, wait_gave_up(t0, kDevTimeoutFull, &sh->abort))) return false;
               }
-              if (!ok) break;
-            } else if (!(ok = wait(&sh->p_full[s][0], par, kDevTimeoutFull))) {
-              break;
+            } else if (!wait(&sh->p_full[s][0], par, kDevTimeoutFull)) {
+              return false;
             }
-            if (!(ok = wait(&sh->v_full[kv.at], kv.phase, kDevTimeoutFull))) break;
             // O += P V in two halves: the first runs under the second's
             // exponentials. The piece's first one overwrites O, which the
             // previous epilogue must hold.
-            if (j == 0 && !(ok = wait(&sh->o_empty[s], o_par >> s & 1, kDevTimeoutFull))) break;
+            const bool first = j < ahead && (wk.dual || j == 0);
+            if (first && !wait(&sh->o_empty[s], o_par >> s & 1, kDevTimeoutFull)) return false;
             tc_fence_after();
             const uint32_t t_p = tbase + C::T_P + C::P_STEP * s, t_o = tbase + C::T_O + HD * s;
-            umma_ts_t64_linear_warp(t_o, t_p, dv, ID_PV, j > 0 ? 1u : 0u);
-            if (!(ok = wait(&sh->p_full[s][1], par, kDevTimeoutFull))) break;
+            umma_ts_t64_linear_warp(t_o, t_p, dv, ID_PV, first ? 0u : 1u);
+            if (!wait(&sh->p_full[s][1], par, kDevTimeoutFull)) return false;
             tc_fence_after();
             umma_ts_t64_linear_warp(t_o, t_p + 32, dv + 512, ID_PV, 1u);
             if (C::OWN_P) umma_commit_warp(&sh->p_empty[s]);
-            if (j + 1 == n_s) umma_commit_warp(&sh->o_full[s]);
-            if (!C::OWN_P && !(ok = next_s())) break;
+            if (j + ahead >= n_s)
+              umma_commit_warp(&sh->o_full[s]);
+            else if (!C::OWN_P && !next_s())
+              return false;
             tile_par ^= 1u << s;
+            return true;
+          };
+          if constexpr (C::OWN_P) {
+#pragma unroll 1
+            for (int s = 0; ok && s < 2; ++s) ok = step(s);
+          } else {
+            ok = step(Const<0>{}) && step(Const<1>{});
           }
           if (!ok) break;
-          umma_commit_warp(&sh->kv_empty[kv.at]);
-          kv = kv1;
+          if (j + ahead < wk.n) umma_commit_warp(&sh->k_empty[kv1.at]);
+          umma_commit_warp(&sh->v_empty[kv.at]);
+          kv.step();
         }
         if (!ok) break;
-        if (wk.n1 == 0 && !(ok = take_any(k + 1, nx))) break;
+        if ((wk.n1 == 0 || wk.dual) && !(ok = take_any(k + 1, nx))) break;
         o_par ^= (uint32_t)(wk.n0 > 0) | (uint32_t)(wk.n1 > 0) << 1;
         wk = nx;
         ++k;
@@ -732,7 +802,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     const int hh = (warp - 4) >> 2;  // big: sub-tile
     const int sub = warp & 3;        // TMEM lane quarter this warp may access
     const int r = sub * 32 + lane;   // query row of the sub-tile
-    const int r_tok = r < p.sub_tokens * p.G ? r / p.G + hh * p.sub_tokens : 0x7fffffff;
+    const int r_tok0 = r < p.sub_tokens * p.G ? r / p.G : 0x40000000;
     const uint32_t lane_bits = (uint32_t)(sub * 32) << 16;
     const uint32_t t_s = tbase + 128 * hh + lane_bits;
     const uint32_t t_p = tbase + C::T_P + C::P_STEP * hh + lane_bits;
@@ -873,11 +943,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       }
       // --------------------------------------------------- big: softmax
       const int n = hh == 0 ? wk.n0 : wk.n1;
+      const int r_tok = r_tok0 + (wk.dual ? 0 : hh * p.sub_tokens);
       // Last visible key. (Rows without a token compute on and are dropped.)
       const int hi = r_tok < wk.ntok ? min(wk.pos0 + r_tok, wk.len - 1) : 0x7fffffff;
       float m_used = -INFINITY, l = 0.f;
       for (int j = 0; j < n; ++j, tile_par ^= 1) {
-        const int kv0 = (wk.k0 + j) * kChunkKeys;
+        const int kv0 = (wk.k0 + (wk.dual ? 2 * j + hh : j)) * kChunkKeys;
         if (!(ok = wait(&sh->s_full[hh], tile_par, kDevTimeoutFull))) break;
         tc_fence_after();
         // S is read twice, 64 columns at a time in rolled loops: once for the
@@ -888,24 +959,28 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const bool masked = __any_sync(0xffffffffu, kv0 + kChunkKeys - 1 > hi);
         // Keys behind the row's last visible one become hugely negative, by
         // arithmetic: the minimum with a line that is huge up to that key and
-        // hugely negative past it (this also drops a NaN score).
+        // hugely negative past it (this also drops a NaN score). The first pass
+        // writes them back for the second.
         const float big = 1.2676506e30f;  // 2^100
         const float hb = (hi >= kv0 ? (float)min(hi - kv0, kChunkKeys - 1) + 0.5f : -1.f) * big;
         auto load = [&](int half, uint32_t(&v)[64]) {
           tmem_ld32(t_s + 64 * half, *reinterpret_cast<uint32_t(*)[32]>(v));
           tmem_ld32(t_s + 64 * half + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
           tmem_wait_ld();
-          if (masked) {
-            const float hbh = hb - (float)(64 * half) * big;
-#pragma unroll
-            for (int e = 0; e < 64; ++e) v[e] = __float_as_uint(fminf(__uint_as_float(v[e]), fmaf(-(float)e, big, hbh)));
-          }
         };
         float mx = -INFINITY;
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {
           uint32_t v[64];
           load(half, v);
+          if (masked) {
+            const float hbh = hb - (float)(64 * half) * big;
+#pragma unroll
+            for (int e = 0; e < 64; ++e) v[e] = __float_as_uint(fminf(__uint_as_float(v[e]), fmaf(-(float)e, big, hbh)));
+            tmem_st32(t_s + 64 * half, *reinterpret_cast<uint32_t(*)[32]>(v));
+            tmem_st32(t_s + 64 * half + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
+            tmem_wait_st();
+          }
           float mp[8];  // independent chains
 #pragma unroll
           for (int q = 0; q < 8; ++q) mp[q] = fmaxf(__uint_as_float(v[q]), __uint_as_float(v[8 + q]));
@@ -965,7 +1040,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               float x0, x1;
               ffma2(x0, x1, __uint_as_float(v[32 * c + e]), __uint_as_float(v[32 * c + e + 1]), p.scale_log2,
                     p.scale_log2, neg_mu, neg_mu);
-              const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+              // One pair in four takes its 2^x on the FMA pipe (relative error
+              // 1e-4, far below the rounding to bf16): the exponentials' own
+              // unit is what both sub-tiles' warps compete for.
+              float p0, p1;
+              if (((e >> 1) & C::FMA_EXP) == C::FMA_EXP) {
+                exp2_fma2(p0, p1, x0, x1);
+              } else {
+                p0 = fast_exp2(x0);
+                p1 = fast_exp2(x1);
+              }
               const int q = 2 * ((e >> 1) & 3);
               fadd2(ls[q], ls[q + 1], ls[q], ls[q + 1], p0, p1);
               pk[e >> 1] = pack_bf16x2(p0, p1);
@@ -981,7 +1065,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       }
       if (!ok) break;
       sh->stats[k & 1][hh][0][r] = m_used;
-      sh->stats[k & 1][hh][1][r] = l;
+      // (exp2_fma2 gives 2^-126, not 0, for a masked key: a row that saw none has no weight.)
+      sh->stats[k & 1][hh][1][r] = m_used == -INFINITY ? 0.f : l;
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->stats_full[k & 1][hh]);
       J += wk.n;
@@ -1060,15 +1145,26 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 #pragma unroll 1
         for (int hh = 0; hh < 2; ++hh) {
           if (hh * p.sub_tokens >= wk.ntok) break;
-          const bool any = (hh == 0 ? wk.n0 : wk.n1) > 0;  // else: no key tile of this piece
-          if (!(ok = sleepy(&sh->stats_full[k & 1][hh], (k >> 1) & 1))) break;
-          if (any) {
-            if (!(ok = sleepy(&sh->o_full[hh], o_par >> hh & 1))) break;
-            o_par ^= 1u << hh;
-            tc_fence_after();
+          // Both sub-tiles' O are the same rows' in a dual piece.
+          const int last = wk.dual ? 1 : hh;
+          for (int s = hh; ok && s <= last; ++s) {
+            ok = sleepy(&sh->stats_full[k & 1][s], (k >> 1) & 1);
+            if (ok && (s == 0 ? wk.n0 : wk.n1) > 0) {  // else: no key tile of this piece
+              ok = sleepy(&sh->o_full[s], o_par >> s & 1);
+              o_par ^= 1u << s;
+            }
           }
-          const float m_used = sh->stats[k & 1][hh][0][r];
-          const float l = sh->stats[k & 1][hh][1][r];
+          if (!ok) break;
+          tc_fence_after();
+          const bool any = (hh == 0 ? wk.n0 : wk.n1) > 0;
+          float m_used = sh->stats[k & 1][hh][0][r], l = sh->stats[k & 1][hh][1][r], f0 = 1.f, f1 = 0.f;
+          if (wk.dual) {
+            const float m1 = sh->stats[k & 1][1][0][r], l1 = sh->stats[k & 1][1][1][r], M = fmaxf(m_used, m1);
+            f0 = l > 0.f ? fast_exp2(m_used - M) : 0.f;
+            f1 = l1 > 0.f ? fast_exp2(m1 - M) : 0.f;
+            m_used = M;
+            l = l * f0 + l1 * f1;
+          }
           const float inv = split ? 1.f : 1.f / l;
           const uint32_t t_o = tbase + C::T_O + HD * hh + lane_bits;
           const int live = min(sub_rows, rows - hh * sub_rows) - sub * 32;  // of this warp's 32 rows
@@ -1082,10 +1178,22 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               uint32_t o[16];
               tmem_ld16(t_o + c, o);
               tmem_wait_ld();
+              if (wk.dual) {
+                uint32_t o1[16];
+                tmem_ld16(t_o + HD + c, o1);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                  o[e] = __float_as_uint((f0 > 0.f ? __uint_as_float(o[e]) * f0 : 0.f) +
+                                         (f1 > 0.f ? __uint_as_float(o1[e]) * f1 : 0.f));
+              }
               if (c == HD - 16 && any) {
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sh->o_empty[hh]);  // the next piece may overwrite O
+                if (lane == 0) {  // the next piece may overwrite O
+                  mbar_arrive(&sh->o_empty[hh]);
+                  if (wk.dual) mbar_arrive(&sh->o_empty[1]);
+                }
               }
 #pragma unroll
               for (int e = 0; e < 16; ++e) o[e] = l > 0.f ? __float_as_uint(__uint_as_float(o[e]) * inv) : 0u;
@@ -1218,6 +1326,7 @@ cudaError_t launch_chunk_plan(const ChunkParams& p, const ChunkLayout& lay, uint
   q.tile_tokens = 2 * p.sub_tokens;
   q.key_limit = p.key_limit;
   q.sms = sms;
+  q.two_subs_cost = chunk_tile_cost(true, p.head_dim);
   q.max_entries = (int)lay.max_entries;
   q.max_slots = (int)lay.max_slots;
   q.entries = reinterpret_cast<ChunkEntry*>(ws + lay.entries);

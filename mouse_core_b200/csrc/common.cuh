@@ -182,15 +182,23 @@ __device__ __noinline__ bool wait_gave_up(uint32_t t0, int code, int* abort) {
   return true;
 }
 
-// mbar_wait_abortable in a compact form; `nap` > 0 sleeps that many nanoseconds
-// between polls, for a wait off the critical path.
-__device__ __forceinline__ bool mbar_wait_or_abort(uint64_t* bar, uint32_t parity, int code, int* abort, int nap) {
+// mbar_wait_abortable in a compact form.
+__device__ __forceinline__ bool mbar_wait_or_abort(uint64_t* bar, uint32_t parity, int code, int* abort) {
   if (mbar_try_wait(bar, parity)) return true;
   const uint32_t t0 = clock32();
   do {
     if (wait_gave_up(t0, code, abort)) return false;
-    if (nap) __nanosleep(nap);
   } while (!mbar_try_wait(bar, parity));
+  return true;
+}
+
+// The same off the critical path: a call, and the warp sleeps between polls.
+__device__ __noinline__ bool mbar_wait_sleepy_or_abort(uint64_t* bar, uint32_t parity, int code, int* abort) {
+  const uint32_t t0 = clock32();
+  while (!mbar_try_wait(bar, parity)) {
+    if (wait_gave_up(t0, code, abort)) return false;
+    __nanosleep(64);
+  }
   return true;
 }
 

@@ -213,6 +213,10 @@ CASES = {
     "group_of_7": ([(100, 50), (1000, 1), (0, 18), (64, 36), (63, 37), (7, 2), (700, 3)], 14, 2, 64, 128),
     "group_of_16": ([(100, 50), (1000, 1), (0, 8), (64, 16), (63, 17), (7, 2)], 16, 1, 128, 192),
     "group_of_32": ([(100, 9), (1000, 1), (0, 4), (64, 8)], 32, 1, 64, 64),
+    "one_sub_tile_even_and_odd_key_tiles": ([(100, 20), (220, 40), (500, 64), (700, 33), (2500, 9), (0, 50), (128, 64)],
+                                            16, 8, 128, 64),
+    "one_sub_tile_hd64": ([(100, 5), (240, 16), (500, 32), (9000, 20), (380, 7), (0, 31)], 32, 8, 64, 64),
+    "one_sub_tile_split": ([(30000, 40), (17, 3)], 16, 8, 128, 128),
     "one_head": ([(0, 5), (600, 1), (128, 128), (127, 257)], 1, 1, 64, 64),
     "long_axis_few_rows": ([(40000, 1), (30001, 3)], 16, 8, 128, 128),
     "long_axis_chunk": ([(20011, 200)], 16, 8, 128, 128),
