@@ -73,9 +73,11 @@ constexpr int kChunkPlanThreads = 1024;
 // Shortest piece: below it a piece's own cost (its queries, its partial, the
 // join) outweighs what another SM gains.
 constexpr int kMinSplitTiles = 4;
-// ... and nothing is gained by pieces shorter than this part of an SM's share of
-// the step: longest first already evens those out.
-constexpr int kPiecesPerShare = 3;
+// ... and little is gained by pieces shorter than an SM's share of the step, or
+// half of it when there are few items: longest first evens those out. (A step
+// of 800 items took 119 us cut at the share and 131 at half of it; 8 items over
+// 131072 keys 199 and 151.)
+constexpr int kManyItems = 4;  // items per SM
 
 // What a key tile costs, in units of half a tile of a small piece or of one with
 // a single sub-tile (both bound by the K/V they read): two sub-tiles' softmax
@@ -111,7 +113,8 @@ __global__ void __launch_bounds__(kChunkPlanThreads) chunk_plan_kernel(const Chu
   __shared__ int hist[kBuckets], warp_tot[32], warp_max[32];
   __shared__ int base_s[kChunkPlanThreads], n_s[kChunkPlanThreads], len_s[kChunkPlanThreads];
   __shared__ int cu_s[kChunkPlanThreads], pre[kChunkPlanThreads + 1];
-  __shared__ unsigned long long warp_sum[32], fit_s[3];
+  __shared__ unsigned long long warp_sum[32];
+  __shared__ unsigned fit_s[3];
   __shared__ int slots_s, splits_s;
   launch_dependents();  // the attention's CTAs set themselves up meanwhile
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, nw = blockDim.x >> 5;
@@ -173,22 +176,24 @@ __global__ void __launch_bounds__(kChunkPlanThreads) chunk_plan_kernel(const Chu
   int hi = max(most, 1);                           // splits nothing, which always fits
   int lo = hi;
   if (room > E) {
-    const unsigned long long share = sum * p.Hkv / (kPiecesPerShare * p.sms);
+    const unsigned long long share = sum * p.Hkv / (p.sms * (E * p.Hkv >= kManyItems * p.sms ? 1 : 2));
     lo = (int)min((unsigned long long)hi, max(max((sum + room - 1) / (unsigned long long)room, share),
                                               (unsigned long long)(2 * kMinSplitTiles)));
+    // c >= sum / (room - E) always fits: pieces are at most sum / c + E.
+    hi = (int)max((unsigned long long)lo, min((unsigned long long)hi, sum / (unsigned long long)(room - E) + 1));
   }
   for (int round = 0; lo < hi; ++round) {
     const int c = (lo + hi) >> 1;
-    unsigned long long pieces = 0;
+    unsigned pieces = 0;
     for (int at = 0; at < p.batch; at += blockDim.x) {
       load(at);
-      for (int t = 0; t < tiles; ++t) pieces += (key_tiles(t) * cost + c - 1) / c;
+      for (int t = 0; t < tiles; ++t) pieces += (unsigned)(key_tiles(t) * cost + c - 1) / c;
     }
-    pieces = warp_add(pieces);
+    pieces = __reduce_add_sync(all, min(pieces, 1u << 21));  // (no sum wraps; so many never fit)
     if (lane == 0 && pieces) atomicAdd(&fit_s[round % 3], pieces);
     if (tid == 0) fit_s[(round + 1) % 3] = 0;  // (read by nobody now: two rounds old)
     __syncthreads();
-    if (fit_s[round % 3] <= (unsigned long long)room)
+    if ((long long)fit_s[round % 3] <= room)
       hi = c;
     else
       lo = c + 1;
@@ -590,7 +595,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               // K and V stages are released apart: K's a tile earlier than V's.
               const bool tail = ragged(k0 + j, len);
               auto load = [&](uint64_t* bar, uint64_t* empty, const CUtensorMap* map, uint8_t* dst) {
-                if (!wait1(empty, kv.phase ^ 1)) return false;
+                if (empty && !wait1(empty, kv.phase ^ 1)) return false;
                 mbar_arrive_expect_tx(bar, C::KVTILE);
 #pragma unroll
                 for (int cb = 0; cb < C::NCB; ++cb) {
@@ -599,9 +604,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 }
                 return true;
               };
-              if (!(ok = load(&sh->k_full[kv.at], &sh->k_empty[kv.at], &kmap, ks + kv.at * C::KVTILE))) break;
+              if (!(ok = load(&sh->k_full[kv.at], C::OWN_P ? &sh->v_empty[kv.at] : &sh->k_empty[kv.at], &kmap,
+                              ks + kv.at * C::KVTILE)))
+                break;
               ++k_issued;
-              if (!(ok = load(tail ? &sh->v_tail[tail_at.at] : &sh->v_full[kv.at], &sh->v_empty[kv.at], &vmap,
+              if (!(ok = load(tail ? &sh->v_tail[tail_at.at] : &sh->v_full[kv.at], C::OWN_P ? nullptr : &sh->v_empty[kv.at], &vmap,
                               vs + kv.at * C::KVTILE)))
                 break;
               kv.step();
@@ -655,7 +662,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           for (int j = 0; j < wk.n; ++j, kv.step(), small_at.step()) {
             if (!(ok = wait(&sh->small_done[small_at.at], small_at.phase, kDevTimeoutFull))) break;
             if (lane == 0) {
-              mbar_arrive(&sh->k_empty[kv.at]);
+              if (!C::OWN_P) mbar_arrive(&sh->k_empty[kv.at]);
               mbar_arrive(&sh->v_empty[kv.at]);
             }
           }
@@ -674,7 +681,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             if (!(ok = wait(&sh->k_full[first.at], first.phase, kDevTimeoutFull))) break;
             issue_qk(s, first.at, q);
           }
-          if (wk.dual || s == 1) umma_commit_warp(&sh->k_empty[first.at]);
+          if (!C::OWN_P && (wk.dual || s == 1)) umma_commit_warp(&sh->k_empty[first.at]);
           if (!wk.dual && n_s <= 1) umma_commit_warp(&sh->q_empty[k & 1][s]);  // its last Q K^T
         }
         if (ok && wk.dual && wk.n <= 2) {
@@ -691,7 +698,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           if (wk.dual) kv1.step();
           const int ahead = wk.dual ? 2 : 1;
           if (!(ok = wait(&sh->v_full[kv.at], kv.phase, kDevTimeoutFull))) break;
-          if (!wk.dual && j + 1 < wk.n && !(ok = wait(&sh->k_full[kv1.at], kv1.phase, kDevTimeoutFull))) break;
+          if (!C::OWN_P && !wk.dual && j + 1 < wk.n && !(ok = wait(&sh->k_full[kv1.at], kv1.phase, kDevTimeoutFull)))
+            break;
           const uint64_t dv = umma_desc_sw128(smem_u32(vs + kv.at * C::KVTILE), C::BOX, 1024);
           // One sub-tile's step: O += P V for tile j and S = Q K^T for its next one.
           // (At head_dim 128 written out for each: the tensor pipe idles while
@@ -703,7 +711,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             if (j >= n_s || (wk.dual && (j & 1) != s)) return true;
             const uint32_t par = tile_par >> s & 1;
             auto next_s = [&]() {
-              if (wk.dual && !wait(&sh->k_full[kv1.at], kv1.phase, kDevTimeoutFull)) return false;
+              if ((C::OWN_P || wk.dual) && !wait(&sh->k_full[kv1.at], kv1.phase, kDevTimeoutFull)) return false;
               issue_qk(s, kv1.at, wk.dual ? 0 : (int)s);
               if (j + ahead + 1 == n_s) {
                 umma_commit_warp(&sh->q_empty[k & 1][s]);
@@ -729,10 +737,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                   if (nx.n0 == 1) umma_commit_warp(&sh->q_empty[(k + 1) & 1][0]);
                   early = true;
                 }
-                if (__all_sync(0xffffffffu, mbar_test_wait(&sh->p_full[1][0], par))) break;
+                if (__all_sync(0xffffffffu, mbar_test_wait(&sh->p_full[1][C::OWN_P], par))) break;
                 if (__any_sync(0xffffffffu, wait_gave_up(t0, kDevTimeoutFull, &sh->abort))) return false;
               }
-            } else if (!wait(&sh->p_full[s][0], par, kDevTimeoutFull)) {
+            } else if (!wait(&sh->p_full[s][C::OWN_P], par, kDevTimeoutFull)) {
               return false;
             }
             // O += P V in two halves: the first runs under the second's
@@ -742,11 +750,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             if (first && !wait(&sh->o_empty[s], o_par >> s & 1, kDevTimeoutFull)) return false;
             tc_fence_after();
             const uint32_t t_p = tbase + C::T_P + C::P_STEP * s, t_o = tbase + C::T_O + HD * s;
-            umma_ts_t64_linear_warp(t_o, t_p, dv, ID_PV, first ? 0u : 1u);
-            if (!wait(&sh->p_full[s][1], par, kDevTimeoutFull)) return false;
-            tc_fence_after();
-            umma_ts_t64_linear_warp(t_o, t_p + 32, dv + 512, ID_PV, 1u);
-            if (C::OWN_P) umma_commit_warp(&sh->p_empty[s]);
+            if constexpr (C::OWN_P) {
+              umma_ts_t128_linear_warp(t_o, t_p, dv, ID_PV, first ? 0u : 1u);
+              umma_commit_warp(&sh->p_empty[s]);
+            } else {
+              umma_ts_t64_linear_warp(t_o, t_p, dv, ID_PV, first ? 0u : 1u);
+              if (!wait(&sh->p_full[s][1], par, kDevTimeoutFull)) return false;
+              tc_fence_after();
+              umma_ts_t64_linear_warp(t_o, t_p + 32, dv + 512, ID_PV, 1u);
+            }
             if (j + ahead >= n_s)
               umma_commit_warp(&sh->o_full[s]);
             else if (!C::OWN_P && !next_s())
@@ -761,7 +773,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             ok = step(Const<0>{}) && step(Const<1>{});
           }
           if (!ok) break;
-          if (j + ahead < wk.n) umma_commit_warp(&sh->k_empty[kv1.at]);
+          if (!C::OWN_P && j + ahead < wk.n) umma_commit_warp(&sh->k_empty[kv1.at]);
           umma_commit_warp(&sh->v_empty[kv.at]);
           kv.step();
         }
@@ -1057,10 +1069,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             tmem_st16(t_p + 32 * half + 16 * c, pk);
           }
           l += ((ls[0] + ls[1]) + (ls[2] + ls[3])) + ((ls[4] + ls[5]) + (ls[6] + ls[7]));
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh->p_full[hh][half]);
+          if (!C::OWN_P || half == 1) {
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->p_full[hh][half]);
+          }
         }
       }
       if (!ok) break;
@@ -1171,6 +1185,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           const size_t pr = part + hh * sub_rows + sub * 32;
           __nv_bfloat16* out = p.out + ((size_t)(wk.q0 + hh * p.sub_tokens) * p.Hq + wk.h * p.G) * HD;
           const int cols = split ? 32 : 64;  // of a 128-byte line
+          // Where this lane's 16 bytes of line c0's eight turned stores go.
+          uint8_t* dst = split ? reinterpret_cast<uint8_t*>(p.part_o + pr * HD + 4 * (lane & 7))
+                               : reinterpret_cast<uint8_t*>(out);
 #pragma unroll 1
           for (int c0 = 0; c0 < HD; c0 += cols) {
 #pragma unroll 1
@@ -1219,12 +1236,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             for (int i = 0; i < 8; ++i) {
               const int row = i * 4 + (lane >> 3);
               const uint4 u = *reinterpret_cast<const uint4*>(stage + row * 128 + (((lane & 7) ^ (row & 7)) << 4));
-              if (row >= live) continue;
-              if (split)
-                *reinterpret_cast<uint4*>(p.part_o + (pr + row) * HD + c0 + 4 * (lane & 7)) = u;
-              else
-                *reinterpret_cast<uint4*>(out + off[i] + c0) = u;
+              if (row < live) *reinterpret_cast<uint4*>(dst + (split ? row * HD * 4 : off[i] * 2)) = u;
             }
+            dst += 128;
             __syncwarp();
           }
           if (split && lane < live) p.part_ml[pr + lane] = make_float2(m_used, l);
