@@ -72,7 +72,8 @@ constexpr int kChunkSmallRows = 16;  // query rows of a small tile (one mma.sync
 constexpr int kChunkPlanThreads = 1024;
 // Shortest piece: below it a piece's own cost (its queries, its partial, the
 // join) outweighs what another SM gains.
-constexpr int kMinSplitTiles = 4;
+// (Costs are in chunk_tile_cost's units: four tiles of the cheaper kind.)
+constexpr int kMinPieceCost = 8;
 // ... and little is gained by pieces shorter than an SM's share of the step, or
 // half of it when there are few items: longest first evens those out. (A step
 // of 800 items took 119 us cut at the share and 131 at half of it; 8 items over
@@ -92,7 +93,7 @@ struct ChunkPlanParams {
   int batch, tokens, G, Hkv, tile_tokens, key_limit, sms, max_entries, max_slots, two_subs_cost;
   ChunkEntry* entries;
   ChunkSplit* splits;
-  int* head;  // [0] entries, [1] next item, [2] CTAs done, [3] splits
+  int* head;  // [0] entries, [1] next item, [2] CTAs done, [3] splits, [4] whether a wait ran out
 };
 
 // Key tiles that query tile t of a row (n new tokens, len cached ones) visits.
@@ -178,7 +179,7 @@ __global__ void __launch_bounds__(kChunkPlanThreads) chunk_plan_kernel(const Chu
   if (room > E) {
     const unsigned long long share = sum * p.Hkv / (p.sms * (E * p.Hkv >= kManyItems * p.sms ? 1 : 2));
     lo = (int)min((unsigned long long)hi, max(max((sum + room - 1) / (unsigned long long)room, share),
-                                              (unsigned long long)(2 * kMinSplitTiles)));
+                                              (unsigned long long)kMinPieceCost));
     // c >= sum / (room - E) always fits: pieces are at most sum / c + E.
     hi = (int)max((unsigned long long)lo, min((unsigned long long)hi, sum / (unsigned long long)(room - E) + 1));
   }
@@ -237,7 +238,7 @@ __global__ void __launch_bounds__(kChunkPlanThreads) chunk_plan_kernel(const Chu
   if (tid == 0) {
     if (!fits) report(kDevBadIndex);
     p.head[0] = fits ? total : 0;
-    p.head[1] = p.head[2] = 0;
+    p.head[1] = p.head[2] = p.head[4] = 0;
   }
   if (!fits) {
     if (tid == 0) p.head[3] = 0;
@@ -390,8 +391,8 @@ struct ChunkRing {
   }
 };
 
-// Masked keys' scores lie below this (-2^90) on the tcgen05 path, where masks
-// are applied by arithmetic; real scores stay far above it.
+// Masked keys' scores lie below this (-2^90) on the tcgen05 path, finite so that
+// a row without a visible key computes no NaN; real scores stay far above it.
 constexpr float kChunkMasked = -1.2379401e27f;
 
 template <int HD>
@@ -969,12 +970,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         // short pieces, where all its roles are busy, a quarter of the fetches
         // missed and tiles took twice as long.)
         const bool masked = __any_sync(0xffffffffu, kv0 + kChunkKeys - 1 > hi);
-        // Keys behind the row's last visible one become hugely negative, by
-        // arithmetic: the minimum with a line that is huge up to that key and
-        // hugely negative past it (this also drops a NaN score). The first pass
-        // writes them back for the second.
-        const float big = 1.2676506e30f;  // 2^100
-        const float hb = (hi >= kv0 ? (float)min(hi - kv0, kChunkKeys - 1) + 0.5f : -1.f) * big;
+        // Scores of the keys behind the row's last visible one, whatever they
+        // are, become hugely negative; the first pass writes them back for the
+        // second.
         auto load = [&](int half, uint32_t(&v)[64]) {
           tmem_ld32(t_s + 64 * half, *reinterpret_cast<uint32_t(*)[32]>(v));
           tmem_ld32(t_s + 64 * half + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
@@ -986,27 +984,28 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           uint32_t v[64];
           load(half, v);
           if (masked) {
-            const float hbh = hb - (float)(64 * half) * big;
+            const int last = hi - kv0 - 64 * half;
 #pragma unroll
-            for (int e = 0; e < 64; ++e) v[e] = __float_as_uint(fminf(__uint_as_float(v[e]), fmaf(-(float)e, big, hbh)));
+            for (int e = 0; e < 64; ++e) v[e] = e <= last ? v[e] : __float_as_uint(2.f * kChunkMasked);
             tmem_st32(t_s + 64 * half, *reinterpret_cast<uint32_t(*)[32]>(v));
             tmem_st32(t_s + 64 * half + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
             tmem_wait_st();
           }
           float mp[8];  // independent chains
 #pragma unroll
-          for (int q = 0; q < 8; ++q) mp[q] = fmaxf(__uint_as_float(v[q]), __uint_as_float(v[8 + q]));
+          for (int q = 0; q < 8; ++q) mp[q] = fmax_nan(__uint_as_float(v[q]), __uint_as_float(v[8 + q]));
 #pragma unroll
           for (int e = 16; e < 64; e += 16)
 #pragma unroll
-            for (int q = 0; q < 8; ++q) mp[q] = fmax3(mp[q], __uint_as_float(v[e + q]), __uint_as_float(v[e + 8 + q]));
-          mx = fmax3(fmax3(mp[0], mp[1], mp[2]), fmax3(mp[3], mp[4], mp[5]), fmax3(mp[6], mp[7], mx));
+            for (int q = 0; q < 8; ++q) mp[q] = fmax3_nan(mp[q], __uint_as_float(v[e + q]), __uint_as_float(v[e + 8 + q]));
+          mx = fmax3_nan(fmax3_nan(mp[0], mp[1], mp[2]), fmax3_nan(mp[3], mp[4], mp[5]), fmax3_nan(mp[6], mp[7], mx));
         }
         // O is rescaled only when the maximum grew by more than 2^8: the final
         // division uses the same stale maximum, so the result is exact. (A row
-        // that sees no key of the tile keeps -inf.)
-        const float m_tile = mx <= kChunkMasked ? -INFINITY : mx * p.scale_log2;
-        const bool grew = m_tile > m_used + 8.f;
+        // that sees no key of the tile keeps -inf; a NaN or +inf among the
+        // visible scores makes the maximum, and with it the row, NaN.)
+        const float m_tile = mx <= kChunkMasked ? -INFINITY : fmaf(mx, p.scale_log2, mx - mx);
+        const bool grew = !(m_tile <= m_used + 8.f);
         // P's columns (and O) are free once the tile before is consumed.
         if (C::OWN_P) {
           if (!(ok = wait(&sh->p_empty[hh], tile_par ^ 1, kDevTimeoutEmpty))) break;
@@ -1016,7 +1015,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           m_used = m_tile;
         } else if (__any_sync(0xffffffffu, grew)) {
           const float alpha = grew ? fast_exp2(m_used - m_tile) : 1.f;
-          if (grew) m_used = m_tile;
+          if (grew) m_used = fmax_nan(m_used, m_tile);  // (NaN stays)
           l *= alpha;
 #pragma unroll 1
           for (int c = 0; c < HD / 16; ++c) {
@@ -1140,7 +1139,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             *reinterpret_cast<float4*>(&p.part_o[(part + rr) * HD + c4 * 4]) = O;
             if (c4 == 0) p.part_ml[part + rr] = make_float2(M, L);
           } else {
-            const float inv = L > 0.f ? 1.f / L : 0.f;
+            const float inv = L != 0.f ? 1.f / L : 0.f;
             const int tok = wk.q0 + rr / p.G, h = wk.h * p.G + rr % p.G;
             uint2 u;
             u.x = pack_bf16x2(O.x * inv, O.y * inv);
@@ -1174,8 +1173,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           float m_used = sh->stats[k & 1][hh][0][r], l = sh->stats[k & 1][hh][1][r], f0 = 1.f, f1 = 0.f;
           if (wk.dual) {
             const float m1 = sh->stats[k & 1][1][0][r], l1 = sh->stats[k & 1][1][1][r], M = fmaxf(m_used, m1);
-            f0 = l > 0.f ? fast_exp2(m_used - M) : 0.f;
-            f1 = l1 > 0.f ? fast_exp2(m1 - M) : 0.f;
+            f0 = l != 0.f ? fast_exp2(m_used - M) : 0.f;
+            f1 = l1 != 0.f ? fast_exp2(m1 - M) : 0.f;
             m_used = M;
             l = l * f0 + l1 * f1;
           }
@@ -1213,7 +1212,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 }
               }
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = l > 0.f ? __float_as_uint(__uint_as_float(o[e]) * inv) : 0u;
+              for (int e = 0; e < 16; ++e) o[e] = l != 0.f ? __float_as_uint(__uint_as_float(o[e]) * inv) : 0u;
               if (split) {
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
@@ -1257,6 +1256,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     __syncwarp();
     tmem_dealloc(tbase, 512);
   }
+  if (threadIdx.x == 0 && *reinterpret_cast<volatile int*>(&sh->abort)) p.head[4] = 1;  // nothing to join until the next plan
 }
 
 // out of the split tiles: over a row's pieces, in their order, M = max m,
@@ -1266,6 +1266,7 @@ __global__ void __launch_bounds__(32 * kJoinRows, 4) chunk_join_kernel(const Chu
   constexpr int E = HD / 32;  // output elements per lane
   wait_for_prior_grid();
   const int lane = threadIdx.x & 31;
+  if (p.head[4]) return;
   const int units = p.head[3] * p.Hkv;
   const size_t step = (size_t)p.Hkv * p.part_rows;
   for (int u = blockIdx.x; u < units; u += gridDim.x) {
@@ -1281,22 +1282,21 @@ __global__ void __launch_bounds__(32 * kJoinRows, 4) chunk_join_kernel(const Chu
     float L = 0.f, o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.f;
-    if (M > -INFINITY) {
+    const float Mu = M == -INFINITY ? 0.f : M;
 #pragma unroll 2
-      for (int c = 0; c < sp.pieces; ++c) {
-        const float2 ml = p.part_ml[first + c * step];
-        const float f = exp2f(ml.x - M);
-        const float* src = p.part_o + (first + c * step) * HD + lane * E;
-        L += ml.y * f;
+    for (int c = 0; c < sp.pieces; ++c) {
+      const float2 ml = p.part_ml[first + c * step];
+      const float f = exp2f(ml.x - Mu);
+      const float* src = p.part_o + (first + c * step) * HD + lane * E;
+      L += ml.y * f;
 #pragma unroll
-        for (int e = 0; e < E; e += 2) {
-          const float2 x = *reinterpret_cast<const float2*>(src + e);
-          o[e] += x.x * f;
-          o[e + 1] += x.y * f;
-        }
+      for (int e = 0; e < E; e += 2) {
+        const float2 x = *reinterpret_cast<const float2*>(src + e);
+        o[e] += x.x * f;
+        o[e + 1] += x.y * f;
       }
     }
-    const float inv = L > 0.f ? 1.f / L : 0.f;
+    const float inv = L != 0.f ? 1.f / L : 0.f;
     __nv_bfloat16* dst = p.out + ((size_t)(sp.q0 + row / p.G) * p.Hq + h * p.G + row % p.G) * HD + lane * E;
 #pragma unroll
     for (int e = 0; e < E; e += 2)
@@ -1319,7 +1319,7 @@ size_t chunk_layout(int batch, int tokens, int Hq, int Hkv, int head_dim, int sm
   lay->max_slots = 2 * extra;
   lay->part_rows = (int)std::min<long long>((long long)tokens * G, tile_tokens * G);
   size_t off = 0;
-  lay->head = off;     off = up(off + 4 * sizeof(int));
+  lay->head = off;     off = up(off + 5 * sizeof(int));
   lay->entries = off;  off = up(off + lay->max_entries * sizeof(ChunkEntry));
   lay->splits = off;   off = up(off + extra * ((lay->part_rows + kJoinRows - 1) / kJoinRows) * sizeof(ChunkSplit));
   lay->part_ml = off;  off = up(off + lay->max_slots * Hkv * lay->part_rows * sizeof(float2));
@@ -1383,8 +1383,9 @@ static cudaError_t launch_chunk(const CUtensorMap& qm, const CUtensorMap& sqm, c
   cfg.attrs = &attr;
   cfg.numAttrs = after_plan ? 1 : 0;
   e = cudaLaunchKernelEx(&cfg, chunk_attention_kernel<HD>, qm, sqm, km, vm, p);
-  // A table too narrow for two pieces needs no join.
-  if (e != cudaSuccess || p.key_limit <= kMinSplitTiles * kChunkKeys) return e;
+  // A table whose longest tile costs no more than the shortest piece allowed needs no join.
+  const long long most = ((long long)p.key_limit + kChunkKeys - 1) / kChunkKeys * chunk_tile_cost(true, HD);
+  if (e != cudaSuccess || most <= kMinPieceCost) return e;
   cfg.gridDim = dim3(8 * grid);
   cfg.blockDim = dim3(32 * kJoinRows);
   cfg.dynamicSmemBytes = 0;

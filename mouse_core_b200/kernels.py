@@ -333,7 +333,10 @@ def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     sees the row's cached slots ``0..p``. Pools ``[P, Hkv, page, hd]`` bf16 (one
     layer, the new tokens' K/V already appended); block_table ``[B, max_pages]``,
     cu_q ``[B + 1]``, kv_len ``[B]`` int32. Returns ``out [T, Hq, hd]``; tokens
-    behind ``cu_q[B]`` are left as they were. ``workspace`` (uint8, at least
+    behind ``cu_q[B]`` are left as they were, and a token with no visible slot
+    gets 0. A NaN in a cached key makes NaN of the tokens that see it; one in a
+    cached value also of those whose last 128-slot tile holds it. Unused slots
+    may hold anything. ``workspace`` (uint8, at least
     ``chunk_workspace_bytes``) is allocated for the call when not given;
     ``plan_ready`` takes the work list that ``chunk_plan`` left in it."""
     _need(q, "q", BF16, contiguous=False)

@@ -403,3 +403,76 @@ def test_other_streams_and_captured_graphs():
     torch.cuda.synchronize()
     assert _status() == 0
     _check(out, _attention_reference(q, kp, vp, table, cu, kv_len, 0.1))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("tiles", [1, 2, 3, 4, 5, 9])
+def test_tables_no_wider_than_their_rows(hd, tiles):
+    """Few rows whose longest tile is split or not, by a table of just the
+    columns that the longest row needs."""
+    _dev()
+    from mouse_core_b200 import kernels as K
+
+    keys = 128 * tiles
+    for i, rows in enumerate(([(0, keys)], [(keys - 64, 64), (3, 1)], [(keys - 1, 1)], [(keys - 100, 90), (0, 20)],
+                              [(0, keys - 84 + 1), (0, 1), (1, 19)])):
+        q, kp, vp, table, cu, kv_len = _paged(rows, 4, 2, hd, 128, seed=tiles + 10 * i)
+        args = q, kp, vp, table[:, :tiles].contiguous(), cu, kv_len, hd ** -0.5
+        out = K.chunk_attention(*args)
+        assert _status() == 0
+        _check(out, _attention_reference(*args), (rows, tiles))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_random_steps(hd):
+    """Rows, lengths, groups and pages drawn at random, rows of every kind in
+    one step."""
+    _dev()
+    from mouse_core_b200 import kernels as K
+
+    rng = np.random.default_rng(hd)
+    for i in range(40):
+        Hkv = int(rng.choice([1, 2, 3, 8]))
+        G = int(rng.choice([1, 2, 3, 4, 5, 8, 16]))
+        page = int(rng.choice([64, 128, 192]))
+        B = int(rng.choice([1, 2, 3, 8, 30]))
+        most_c, most_n = int(rng.choice([1, 200, 5000])), int(rng.choice([1, 4, 40, 300]))
+        rows = [(int(rng.integers(0, most_c + 1)), int(rng.integers(0, most_n + 1))) for _ in range(B)]
+        rows[0] = (rows[0][0], most_n)
+        args = (*_paged(rows, Hkv * G, Hkv, hd, page, seed=i), hd ** -0.5)
+        out = K.chunk_attention(*args)
+        assert _status() == 0
+        _check(out, _attention_reference(*args), (i, Hkv, G, page, rows))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_what_a_token_sees_decides_whether_its_output_is_a_number(hd, bad):
+    """A NaN (or an infinity whose scores are NaN or +inf) in one cached key
+    makes NaN of the tokens that see it and leaves the others as they are, in
+    every kind of tile; so does one in a token's query."""
+    _dev()
+    from mouse_core_b200 import kernels as K
+
+    # (cached, new, position of the bad key): single tokens, one sub-tile, two, split rows.
+    rows = [(700, 1, 90), (300, 40, 320), (100, 300, 250), (20000, 1, 3), (15000, 100, 15030), (64, 2, None)]
+    q, kp, vp, table, cu, kv_len = _paged([r[:2] for r in rows], 8, 4, hd, 64, seed=hd)
+    q[:, :, 0] = 1.0  # so that +inf in a key's first element is a score of +inf
+    clean = kp.clone()
+    for b, (_, _, at) in enumerate(rows):
+        if at is not None:
+            kp[table[b, at // 64], :, at % 64, 0] = bad
+    q[-1, 3] = float("nan")
+    out = K.chunk_attention(q, kp, vp, table, cu, kv_len, 0.1)
+    assert _status() == 0
+    zeroed = q.clone()
+    zeroed[-1, 3] = 0.0
+    o, A = _attention_reference(zeroed, clean, vp, table, cu, kv_len, 0.1)
+    sees = torch.zeros(q.shape[:2], dtype=torch.bool, device="cuda")
+    for b, (c, n, at) in enumerate(rows):
+        if at is not None:
+            t = torch.arange(c, c + n, device="cuda")
+            sees[cu[b]:cu[b + 1]] = (t >= at)[:, None]
+    sees[-1, 3] = True
+    assert bool(torch.isnan(out[sees].float()).all())
+    _check(out[~sees], (o[~sees], A[~sees]))
