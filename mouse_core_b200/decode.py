@@ -23,6 +23,11 @@ What changes is the machinery, built for B200:
   copy; the split-KV work list is built once on the device and reused by every
   layer. The reference's host syncs (``.max()`` at flex_decode.py:180,
   ``nonzero`` at :195) are gone.
+* A call whose rows bring chunks of very different lengths can skip the
+  left-padding (flex_decode.py:186-198 pads every row to the longest):
+  ``forward_packed`` takes the new tokens of all rows as one ``[T, D]`` stream,
+  K14 makes positions, slots and table entries on the device and K15 attends
+  from each row's chunk to its cached pages.
 
 The session requires a CUDA bf16 model with head_dim 64 or 128; anything else
 raises — there is no CPU or eager fallback.
@@ -177,6 +182,8 @@ class PagedDecodeSession:
         self._len = np.zeros(self.B, dtype=np.int64)
         self._bt_dev = torch.full((self.B, self.pages.max_pages), -1, dtype=torch.int32, device=self.device)
         self._workspace = torch.empty(0, dtype=torch.uint8, device=self.device)
+        # forward_packed's own, so that its growth leaves captured graphs valid.
+        self._chunk_workspace = torch.empty(0, dtype=torch.uint8, device=self.device)
         self._meta_dev = torch.empty(0, dtype=torch.int32, device=self.device)
         # Single-token steps (S = 1, the steady state of env stepping) replay a
         # CUDA graph of the whole layer stack after one eager warm-up call.
@@ -239,6 +246,7 @@ class PagedDecodeSession:
         c._meta_dev = self._meta_dev.clone()
         c._new_page_dev = self._new_page_dev.clone()
         c._workspace = torch.empty_like(self._workspace)
+        c._chunk_workspace = torch.empty_like(self._chunk_workspace)
         c._graph = c._graph_key = c._step_graph = c._step_graph_key = c._step_args = None
         c._graph_warm = c._step_graph_warm = False
         c._step_ids = c._step_out = None
@@ -246,22 +254,29 @@ class PagedDecodeSession:
         c.attn_events = None
         return c
 
-    def _attend(self, q, li, scale, q_pos, kv_len, split):
+    def _attend(self, q, li, scale, q_pos, kv_len, split, cu_q=None):
         """Attention of layer ``li`` over the page pool (K1 split/block decode
-        or the tcgen05 paged prefill). With ``attn_events`` set, the launch is
+        or the tcgen05 paged prefill; K15 for a packed stream with row offsets
+        ``cu_q``). With ``attn_events`` set, the launch is
         then repeated ``attn_reps`` times between two CUDA events on the
         launching stream: each repeat is queued behind the previous launch,
         so the events time the kernel and not a gap while the host submits it
         (the launch reads the pools and writes a fresh output: repeats are
         idempotent)."""
-        args = (q, self.k_pool[li], self.v_pool[li], self._bt_dev, q_pos, kv_len, scale, self.cap)
-        o = K.decode_attention(*args, workspace=self._workspace, plan_ready=split)
+        if cu_q is not None:
+            run, split, workspace = K.chunk_attention, True, self._chunk_workspace
+            args = (q, self.k_pool[li], self.v_pool[li], self._bt_dev, cu_q, kv_len, scale)
+        else:
+            run, workspace = K.decode_attention, self._workspace
+            args = (q.view(self.B, -1, *q.shape[1:]), self.k_pool[li], self.v_pool[li], self._bt_dev, q_pos, kv_len,
+                    scale, self.cap)
+        o = run(*args, workspace=workspace, plan_ready=split)
         if self.attn_events is not None:
             reps = max(1, int(self.attn_reps))
             ev0, ev1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
             ev0.record()
             for _ in range(reps):
-                o = K.decode_attention(*args, workspace=self._workspace, plan_ready=split)
+                o = run(*args, workspace=workspace, plan_ready=split)
             ev1.record()
             self.attn_events.append((ev0, ev1, reps))
         return o
@@ -566,6 +581,83 @@ class PagedDecodeSession:
         K._count(self._graph_launches)
         return self._final(self._graph_out.view(B, S, D), copy=True)
 
+    def prepare_packed(self, lengths, tokens: int):
+        """Host bookkeeping of one packed call: allocate pages and upload the
+        chunk and cached lengths with the opened pages' ids (and the whole
+        block table when the device copy is stale) in one copy; K14 makes the
+        rest on the device. Returns the device views ``(q_pos [T], kv_len [B],
+        slot [T], cu_q [B + 1])``."""
+        B, pages = self.B, self.pages
+        n = np.asarray(lengths, dtype=np.int64).reshape(-1)
+        if n.shape[0] != B:
+            raise ValueError(f"lengths has {n.shape[0]} entries, session batch_size={B}.")
+        if (n < 0).any() or int(n.sum()) != tokens:
+            raise ValueError(f"lengths must be >= 0 and sum to the {tokens} packed tokens.")
+        new_len = self._len + n
+        add = pages.pages_needed(new_len)
+        total = int(add.sum())
+        if total > pages.free_pages:
+            self._grow_pool(total)
+        stale = pages.dirty or bool(self._pending_reset.any()) or self._bt_dev.shape[1] != pages.max_pages
+        ids = pages.open_chunks(add)
+        width = pages.max_pages
+        stale = stale or self._bt_dev.shape[1] != width
+        n_meta = 2 * B + total + (B * width if stale else 0)
+        buf, i = self._stage(n_meta)
+        host = buf.numpy()
+        host[:B] = n
+        host[B:2 * B] = self._len
+        host[2 * B:2 * B + total] = ids
+        if stale:
+            host[2 * B + total:n_meta] = pages.table.reshape(-1)
+        dev = buf[:n_meta].to(self.device, non_blocking=True)
+        ev = self._staging_ev[i]
+        if ev is None:
+            ev = self._staging_ev[i] = torch.cuda.Event()
+        ev.record()
+        if stale:
+            if self._bt_dev.shape[1] != width:
+                self._bt_dev = torch.empty((B, width), dtype=torch.int32, device=self.device)
+            self._bt_dev.copy_(dev[2 * B + total:].view(B, width))
+            pages.dirty = False
+            self._pending_reset[:] = False
+        cu_q, q_pos, slot, kv_len, _ = K.chunk_meta(dev[:B], dev[B:2 * B], self._bt_dev, dev[2 * B:2 * B + total],
+                                                    self.page_size, tokens)
+        self._len = new_len
+        self._device_step_ok = False  # K8's buffers still hold the step before
+        return q_pos, kv_len, slot, cu_q
+
+    @torch.no_grad()
+    def forward_packed(self, *, embeds: torch.Tensor, lengths, output_hidden_states: bool = False):
+        """Decode one chunk per sequence without padding: ``embeds [T, D]``
+        holds the rows' new tokens one row after the other, ``lengths[b]`` of
+        row ``b`` (zero included; their sum is ``T``). Returns hidden states
+        ``[T, D]`` in the same order and, with ``output_hidden_states=True``,
+        the tuple of per-layer hidden states.
+
+        The cache, ``reset_rows`` and ``fork`` are those of ``forward``; calls
+        of both kinds may follow one another in any order. Every GEMM, norm and
+        attention tile works on real tokens only, so a call that mixes long
+        chunks with single tokens costs what its tokens cost, where ``forward``
+        costs ``B`` times its longest chunk. The lengths are read on the host,
+        so the call cannot be captured into a CUDA graph."""
+        if embeds.ndim != 2 or embeds.shape[1] != self.model.config.hidden_size:
+            raise ValueError("forward_packed takes embeds [T, hidden_size], the rows' new tokens one row after the "
+                             f"other; got {tuple(embeds.shape)}")
+        with nvtx_range("packed_step"), torch.cuda.device(self.device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("forward_packed reads lengths on the host and cannot be captured")
+            T = embeds.shape[0]
+            x = embeds.to(self.device, self.dtype).contiguous()
+            q_pos, kv_len, slot, cu_q = self.prepare_packed(lengths, T)
+            if T == 0:
+                return (x, tuple(x for _ in range(self.n_layers))) if output_hidden_states else x
+            out = self._body(x, q_pos, kv_len, slot, 0, output_hidden_states, cu_q)
+            if output_hidden_states:
+                h, hiddens = out
+                return self._final(h), tuple(t.to(self.dtype) for t in hiddens)
+            return self._final(out)
+
     def _final(self, h: torch.Tensor, copy: bool = False) -> torch.Tensor:
         """The model's final norm, in the model's dtype (a fresh tensor when
         ``h`` is a graph buffer)."""
@@ -658,14 +750,15 @@ class PagedDecodeSession:
         K._count(self._step_launches)
         return self._step_out
 
-    def _body(self, x, q_pos, kv_len, slot, S, output_hidden_states):
-        """The layer stack for flattened ``x [B*S, D]``; returns the last hidden
-        state (before the final norm) and, if asked, every layer's."""
+    def _body(self, x, q_pos, kv_len, slot, S, output_hidden_states, cu_q=None):
+        """The layer stack for flattened ``x [B*S, D]`` (or, with row offsets
+        ``cu_q``, a packed ``x [T, D]``); returns the last hidden state (before
+        the final norm) and, if asked, every layer's."""
         if self.residual_fp32:
-            return self._body_f32(x, q_pos, kv_len, slot, S, output_hidden_states)
-        B = self.B
+            return self._body_f32(x, q_pos, kv_len, slot, S, output_hidden_states, cu_q)
+        T = x.shape[0]
         Hq, Hkv, hd = self.n_heads, self.n_kv_heads, self.head_dim
-        split = self._plan(kv_len, S)
+        split = self._plan(kv_len, S) if cu_q is None else self._chunk_plan(cu_q, kv_len, T)
         q_pos_flat = q_pos.reshape(-1)
 
         resid, delta = x, None
@@ -680,8 +773,8 @@ class PagedDecodeSession:
             q = K.kv_append(qkv, q_pos_flat, Hq, Hkv, hd, self.inv_freq, self.attention_scaling,
                             lw.q_norm_w, lw.k_norm_w, lw.qk_eps, slot=slot,
                             k_pool=self.k_pool[li], v_pool=self.v_pool[li])
-            o = self._attend(q.view(B, S, Hq, hd), li, lw.scale, q_pos, kv_len, split)
-            a = lw.o_proj(o.view(B * S, Hq * hd))
+            o = self._attend(q, li, lw.scale, q_pos, kv_len, split, cu_q)
+            a = lw.o_proj(o.view(T, Hq * hd))
             resid, hn2 = K.rmsnorm(a, lw.post_w, lw.post_eps, residual=resid)
             delta = lw.down(K.silu_mul(F.linear(hn2, lw.wgu, lw.bgu)))
             if output_hidden_states:
@@ -712,6 +805,15 @@ class PagedDecodeSession:
             self._step_graph = None
         return split
 
+    def _chunk_plan(self, cu_q, kv_len, tokens: int) -> bool:
+        """K15's work list for a packed call (once, shared by every layer)."""
+        Hq, Hkv, hd = self.n_heads, self.n_kv_heads, self.head_dim
+        need = K.chunk_workspace_bytes(self.B, tokens, Hq, Hkv, hd)
+        if self._chunk_workspace.numel() < need:
+            self._chunk_workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
+        K.chunk_plan(cu_q, kv_len, tokens, Hq, Hkv, hd, self.page_size, self._bt_dev.shape[1], self._chunk_workspace)
+        return True
+
     def _fused_qkv(self, lw, tokens: int) -> bool:
         """Whether this layer's QKV projection runs as K13: asked for
         (``fused_qkv``), bf16 weights (and norms and bias), heads filling whole
@@ -723,7 +825,7 @@ class PagedDecodeSession:
             return False
         return all(t is None or t.dtype == torch.bfloat16 for t in (lw.bqkv, lw.q_norm_w, lw.k_norm_w))
 
-    def _body_f32(self, x, q_pos, kv_len, slot, S, output_hidden_states):
+    def _body_f32(self, x, q_pos, kv_len, slot, S, output_hidden_states, cu_q=None):
         """The layer stack with an fp32 residual stream: the embeddings enter
         it exactly, every residual add and every projection output stays
         fp32 (cuBLAS bf16 GEMMs with fp32 outputs), and only the GEMM inputs
@@ -733,9 +835,9 @@ class PagedDecodeSession:
         every add and every op output instead; against the fp32 forward this
         path's greedy actions agree more often (measured on the decode
         benchmark's model shape). Returns fp32 hidden states."""
-        B = self.B
+        T = x.shape[0]
         Hq, Hkv, hd = self.n_heads, self.n_kv_heads, self.head_dim
-        split = self._plan(kv_len, S)
+        split = self._plan(kv_len, S) if cu_q is None else self._chunk_plan(cu_q, kv_len, T)
         q_pos_flat = q_pos.reshape(-1)
         resid, delta = None, None
         hiddens = []
@@ -746,7 +848,7 @@ class PagedDecodeSession:
                 resid, hn = K.rmsnorm_f32(x, lw.in_w, lw.in_eps)
             else:
                 resid, hn = K.rmsnorm_f32(resid, lw.in_w, lw.in_eps, delta=delta, sum_out=resid)
-            if self._fused_qkv(lw, B * S):
+            if self._fused_qkv(lw, T):
                 # K13: the QKV GEMM with K2 as its epilogue; one RoPE table
                 # for the step's tokens serves every layer.
                 if rope is None:
@@ -758,8 +860,8 @@ class PagedDecodeSession:
                 q = K.kv_append(qkv, q_pos_flat, Hq, Hkv, hd, self.inv_freq, self.attention_scaling,
                                 lw.q_norm_w, lw.k_norm_w, lw.qk_eps, slot=slot,
                                 k_pool=self.k_pool[li], v_pool=self.v_pool[li])
-            o = self._attend(q.view(B, S, Hq, hd), li, lw.scale, q_pos, kv_len, split)
-            a = _mm_f32(o.view(B * S, Hq * hd), lw.o_proj.weight, lw.o_proj.bias)
+            o = self._attend(q, li, lw.scale, q_pos, kv_len, split, cu_q)
+            a = _mm_f32(o.view(T, Hq * hd), lw.o_proj.weight, lw.o_proj.bias)
             resid, hn2 = K.rmsnorm_f32(resid, lw.post_w, lw.post_eps, delta=a, sum_out=resid)
             delta = _mm_f32(K.silu_mul_f32(_mm_f32(hn2, lw.wgu, lw.bgu)), lw.down.weight, lw.down.bias)
             if output_hidden_states:

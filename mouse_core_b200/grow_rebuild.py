@@ -27,7 +27,10 @@ models/base.py:932-934.
 A rebuilt row and the appended rows of the same call go through ONE ragged
 ``forward`` (the rebuilt rows are emptied first, then receive their window as
 a left-padded chunk), so a call is one pass over the layer stack whatever
-mix of appends and rebuilds it holds. Steps are tokens here (one token per
+mix of appends and rebuilds it holds. With ``packed=True`` that call is
+``forward_packed``: the rows' new tokens in one stream without padding, so one
+row's window of ``start_cache`` tokens no longer makes every other row's single
+token cost as much. Steps are tokens here (one token per
 step, as in the decode benchmark's transition tokens).
 """
 
@@ -54,11 +57,14 @@ class GrowRebuildDecoder:
             ``resolve_cache_bounds`` (kv_policy.py:14-29).
         per_row: Rebuild only the rows that need it (see the module docstring).
         page_size / num_pages: Passed to the session.
+        packed: Run calls that give a row more than one token without padding
+            (``PagedDecodeSession.forward_packed``); ``step`` then returns the
+            hidden states as one packed ``[sum(fed), D]`` stream.
     """
 
     def __init__(self, backbone, batch_size: int, embed: Callable[[torch.Tensor], torch.Tensor], *, max_cache: int,
                  start_cache: int | None = None, per_row: bool = False, page_size: int = 128,
-                 num_pages: int | None = None) -> None:
+                 num_pages: int | None = None, packed: bool = False) -> None:
         self.backbone = backbone
         self.B = int(batch_size)
         self.embed = embed
@@ -66,6 +72,7 @@ class GrowRebuildDecoder:
         self.per_row = bool(per_row)
         self.page_size = int(page_size)
         self.num_pages = num_pages
+        self.packed = bool(packed)
         self.session = None
         self.cached_starts = np.zeros(self.B, dtype=np.int64)
         self.cached_ends = np.zeros(self.B, dtype=np.int64)
@@ -164,7 +171,9 @@ class GrowRebuildDecoder:
             is each fed row's latest hidden state) and ``fed [B]``, the tokens
             each row received (0 for a row with nothing new or an emptied
             context). With ``output_hidden_states`` the session's per-layer
-            tuple is returned as a third element.
+            tuple is returned as a third element. With ``packed`` every hidden
+            state is ``[sum(fed), D]`` instead, row after row, and ``head``'s
+            output is meaningless for rows that received nothing.
         """
         B = self.B
         hist = np.asarray(history)
@@ -189,6 +198,10 @@ class GrowRebuildDecoder:
             self.rows_rebuilt += int(rows.size)
         fed = np.maximum(ends - starts, 0)
         S = max(int(fed.max()) if B else 0, 1)
+        if S > 1 and self.packed:
+            out = self._packed_step(hist, starts, fed, head, output_hidden_states)
+            self.cached_ends = ends.copy()
+            return out
         if S == 1:
             ids = hist[np.arange(B), np.maximum(ends - 1, 0)][:, None]
         else:
@@ -205,7 +218,31 @@ class GrowRebuildDecoder:
             return out, fed
         out = self.session.forward(embeds=self.embed(ids_dev), lengths=fed, output_hidden_states=output_hidden_states)
         self.cached_ends = ends.copy()
+        if self.packed:  # one token per row at most: keep the rows that received one
+            live = np.flatnonzero(fed)
+            at = None if live.size == B else self._stage_ids(live.astype(np.int32))
+
+            def pack(h):
+                return h[:, -1] if at is None else h[:, -1].index_select(0, at)
+
+            out = (pack(out[0]), tuple(pack(h) for h in out[1])) if output_hidden_states else pack(out)
         if output_hidden_states:
             h, hiddens = out
             return h, fed, hiddens
         return out, fed
+
+    def _packed_step(self, hist, starts, fed, head, output_hidden_states):
+        """A call in which some row receives more than one token, as one packed
+        stream: the ids of ``hist[b, starts[b]:starts[b] + fed[b]]`` row after
+        row and the index of each row's latest token go up in one copy."""
+        offsets = np.cumsum(fed) - fed
+        T = int(fed.sum())
+        rows = np.repeat(np.arange(self.B), fed)
+        cols = np.arange(T) + np.repeat(starts - offsets, fed)
+        last = np.maximum(offsets + fed - 1, 0)
+        dev = self._stage_ids(np.concatenate([hist[rows, cols], last]).astype(np.int32))
+        out = self.session.forward_packed(embeds=self.embed(dev[:T]), lengths=fed,
+                                          output_hidden_states=output_hidden_states)
+        if output_hidden_states:
+            return out[0], fed, out[1]
+        return (out if head is None else head(out.index_select(0, dev[T:]))), fed

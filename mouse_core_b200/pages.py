@@ -72,10 +72,17 @@ class PageTable:
 
     def allocate(self, add: np.ndarray) -> None:
         """Append ``add[b]`` fresh pages to row ``b`` (enough must be free)."""
+        if self.open_chunks(add).size:
+            self.dirty = True
+
+    def open_chunks(self, add: np.ndarray) -> np.ndarray:
+        """``allocate``, returning the fresh ids row by row. ``dirty`` is left
+        as it is unless the table had to widen: the caller writes the new
+        entries into the device table."""
         add = np.asarray(add, dtype=np.int64)
         total = int(add.sum())
         if total == 0:
-            return
+            return np.empty(0, dtype=np.int32)
         if total > self._nfree:
             raise RuntimeError(f"page pool exhausted: need {total} pages, {self._nfree} free")
         self.ensure_width(int((self.npages + add).max()))
@@ -87,7 +94,7 @@ class PageTable:
         self.table[rows, starts + offs] = ids
         self.refcount[ids] += 1
         self.npages += add
-        self.dirty = True
+        return ids
 
     def open_pages(self, rows: np.ndarray) -> np.ndarray:
         """Append one fresh page to each of ``rows`` (distinct, ascending; the

@@ -1,0 +1,62 @@
+"""Host side of the packed decode call (no GPU): the page allocator's
+``open_chunks``, which pages a call opens and in which order, and every
+refusal of ``forward_packed`` before anything reaches the device."""
+
+from __future__ import annotations
+
+from types import SimpleNamespace
+
+import numpy as np
+import pytest
+import torch
+
+from mouse_core_b200.decode import PagedDecodeSession
+from mouse_core_b200.pages import PageTable
+
+
+@pytest.mark.parametrize("add", [[0, 0, 0], [1, 0, 2], [0, 5, 1]])
+def test_open_chunks_is_allocate_without_the_dirty_mark(add):
+    a, b = PageTable(3, 8, 64, 6), PageTable(3, 8, 64, 6)
+    a.dirty = b.dirty = False
+    ids = a.open_chunks(np.array(add))
+    b.allocate(np.array(add))
+    assert (a.table == b.table).all() and (a.npages == b.npages).all() and (a.refcount == b.refcount).all()
+    assert a.free_pages == b.free_pages
+    assert not a.dirty and b.dirty == (sum(add) > 0)
+    # Handed out row by row, as the device writes them into its table.
+    assert ids.tolist() == [int(i) for r in range(3) for i in a.table[r, :add[r]]]
+
+
+def test_open_chunks_marks_a_widened_table_and_refuses_an_empty_pool():
+    t = PageTable(2, 6, 64, 1)
+    t.dirty = False
+    t.open_chunks(np.array([3, 0]))
+    assert t.dirty and t.max_pages >= 3
+    with pytest.raises(RuntimeError, match="exhausted"):
+        t.open_chunks(np.array([0, 4]))
+    assert t.free_pages == 3 and t.npages.tolist() == [3, 0]
+
+
+def _stub():
+    s = object.__new__(PagedDecodeSession)
+    s.B, s.page_size, s.n_layers = 3, 64, 1
+    s.device, s.dtype = torch.device("cpu"), torch.bfloat16
+    s.model = SimpleNamespace(config=SimpleNamespace(hidden_size=16))
+    s.pages = PageTable(3, 8, 64, 2)
+    s._len = np.array([0, 5, 64])
+    return s
+
+
+@pytest.mark.parametrize("embeds", [torch.zeros(3, 1, 16), torch.zeros(16), torch.zeros(4, 8)])
+def test_forward_packed_refuses_other_layouts(embeds):
+    with pytest.raises(ValueError, match="hidden_size"):
+        _stub().forward_packed(embeds=embeds, lengths=[1, 2, 1])
+
+
+@pytest.mark.parametrize("lengths", [[1, 3], [1, 3, 0, 0], [5, -1, 0], [1, 1, 1], [4, 1, 0]])
+def test_prepare_packed_refuses_lengths_that_do_not_fit(lengths):
+    s = _stub()
+    with pytest.raises(ValueError, match="lengths"):
+        s.prepare_packed(lengths, 4)
+    # Nothing was allocated or advanced by a refused call.
+    assert s.pages.free_pages == 8 and s._len.tolist() == [0, 5, 64] and s.pages.npages.tolist() == [0, 0, 0]
