@@ -1384,7 +1384,8 @@ static cudaError_t launch_chunk(const CUtensorMap& qm, const CUtensorMap& sqm, c
   cfg.numAttrs = after_plan ? 1 : 0;
   e = cudaLaunchKernelEx(&cfg, chunk_attention_kernel<HD>, qm, sqm, km, vm, p);
   // A table whose longest tile costs no more than the shortest piece allowed needs no join.
-  const long long most = ((long long)p.key_limit + kChunkKeys - 1) / kChunkKeys * chunk_tile_cost(true, HD);
+  const long long most = ((long long)p.key_limit + kChunkKeys - 1) / kChunkKeys *
+                         chunk_tile_cost(p.tokens > p.sub_tokens, HD);
   if (e != cudaSuccess || most <= kMinPieceCost) return e;
   cfg.gridDim = dim3(8 * grid);
   cfg.blockDim = dim3(32 * kJoinRows);

@@ -252,6 +252,16 @@ def decode_step_meta_launch(args: tuple, use_new_page: bool, stream: int) -> Non
     _count()
 
 
+def _all_on(dev: int, dtype, *tensors) -> bool:
+    """Whether every argument is a contiguous tensor of ``dtype`` on CUDA device
+    ``dev``: the good case in one pass, for calls whose time is the host's;
+    ``_check_on`` says what is wrong."""
+    for t in tensors:
+        if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == dev >= 0 and t.is_contiguous()):
+            return False
+    return True
+
+
 def _check_on(dev: int, dtype, **tensors) -> None:
     """Every tensor (``None`` is skipped) is contiguous, of ``dtype`` and on CUDA device ``dev``."""
     for name, t in tensors.items():
@@ -281,19 +291,20 @@ def chunk_meta(lengths: torch.Tensor, kv_len: torch.Tensor, block_table: torch.T
     from ``free_pages``). A step that does not fit is reported through
     ``_lib.device_status`` (3: out of pages or table columns, 7: out of
     tokens) and its tokens without a page get slot -1."""
-    _need(lengths, "lengths", torch.int32)
-    dev = lengths.get_device()
-    _check_on(dev, torch.int32, kv_len=kv_len, block_table=block_table, free_pages=free_pages)
+    dev = lengths.get_device() if isinstance(lengths, torch.Tensor) else -1
+    if not _all_on(dev, torch.int32, lengths, kv_len, block_table, free_pages):
+        _need(lengths, "lengths", torch.int32)
+        _check_on(dev, torch.int32, kv_len=kv_len, block_table=block_table, free_pages=free_pages)
     B, T = lengths.numel(), int(n_tokens)
     if lengths.ndim != 1 or kv_len.shape != lengths.shape or block_table.ndim != 2 or block_table.shape[0] != B:
         raise ValueError("lengths and kv_len must be [B] and block_table [B, max_pages]")
     if T < 0 or page_size <= 0:
         raise ValueError("n_tokens must be >= 0 and page_size > 0")
-    if torch.cuda.current_device() != dev:
+    if torch._C._cuda_getDevice() != dev:
         with torch.cuda.device(dev):
             return chunk_meta(lengths, kv_len, block_table, free_pages, page_size, n_tokens)
-    buf = torch.empty(3 * B + 2 + 2 * T, dtype=torch.int32, device=lengths.device)
-    cu_q, cu_pages, new_len, q_pos, slot = buf.split_with_sizes((B + 1, B + 1, B, T, T))
+    buf = lengths.new_empty(3 * B + 2 + 2 * T)
+    cu_q, cu_pages, new_len, q_pos, slot = buf.unsafe_split_with_sizes((B + 1, B + 1, B, T, T))
     at = buf.data_ptr()
     _lib.call("mb_chunk_meta", lengths.data_ptr(), kv_len.data_ptr(), B, block_table.data_ptr(), block_table.shape[1],
               page_size, free_pages.data_ptr(), free_pages.numel(), T, at, at + 4 * (B + 1), at + 8 * (B + 1),
@@ -339,10 +350,13 @@ def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     may hold anything. ``workspace`` (uint8, at least
     ``chunk_workspace_bytes``) is allocated for the call when not given;
     ``plan_ready`` takes the work list that ``chunk_plan`` left in it."""
-    _need(q, "q", BF16, contiguous=False)
-    dev = q.get_device()
-    _check_on(dev, BF16, k_pool=k_pool, v_pool=v_pool, out=out)
-    _check_on(dev, torch.int32, block_table=block_table, cu_q=cu_q, kv_len=kv_len)
+    dev = q.get_device() if isinstance(q, torch.Tensor) and q.dtype is BF16 else -1
+    if not (_all_on(dev, BF16, k_pool, v_pool) and _all_on(dev, torch.int32, block_table, cu_q, kv_len)):
+        _need(q, "q", BF16, contiguous=False)
+        _check_on(dev, BF16, k_pool=k_pool, v_pool=v_pool)
+        _check_on(dev, torch.int32, block_table=block_table, cu_q=cu_q, kv_len=kv_len)
+    if out is not None:
+        _check_on(dev, BF16, out=out)
     if q.ndim != 3 or k_pool.ndim != 4 or k_pool.shape != v_pool.shape:
         raise ValueError("q must be [T, Hq, hd] and the pools [P, Hkv, page, hd] of equal shape")
     T, Hq, hd = q.shape
@@ -361,7 +375,7 @@ def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         _check_on(dev, torch.uint8, workspace=workspace)
     elif plan_ready:
         raise ValueError("plan_ready needs the workspace that holds the plan")
-    if torch.cuda.current_device() != dev:
+    if torch._C._cuda_getDevice() != dev:
         with torch.cuda.device(dev):
             return chunk_attention(q, k_pool, v_pool, block_table, cu_q, kv_len, scale, out, workspace, plan_ready)
     if out is None:
