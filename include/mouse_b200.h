@@ -52,7 +52,8 @@ int mb_version(void);
  * id outside the pool (or a token past the block table); 4 = misaligned
  * dynamic shared memory; 5 = a stored-dS pair index outside the scratch;
  * 6 = a CTA's own copies or MMAs did not complete before it exited; 7 = an embedding id
- * outside its table, or a TD action / done code out of range. */
+ * outside its table, a TD action / done code out of range, a ragged step of
+ * more tokens than its stream holds, or a work list made for other sizes. */
 int mb_device_status(int* status_out, int clear);
 
 /* Diagnostics, no counterpart in the reference (whose kernels come from
@@ -259,12 +260,16 @@ int mb_chunk_meta(const int32_t* lengths, const int32_t* kv_len, int batch, int3
  * of 8; scale > 0. Slots of a page behind the row's last token are not read
  * as values (they may hold NaN). A page id outside the pool reads as zeros
  * and sets status 3, as does a kv_len beyond max_pages * page_size (the keys
- * past the table are left out); offsets that overlap set status 7 and write
- * nothing.
+ * past the table are left out). Offsets must not decrease: a decreasing pair
+ * is an empty row, and rows that overlap write the same entries of out in no
+ * order, or set status 7 and write nothing when they ask for more tiles than
+ * the stream holds. A NaN in a cached key makes NaN of the tokens that see it;
+ * one in a cached value also of those whose last 128-slot tile holds it.
  *
  * mb_chunk_plan builds the step's work list in `workspace` from cu_q and
  * kv_len alone, so one plan serves every layer of a step: pass plan_ready = 1
- * with the same sizes; 0 builds it in the call. Needs
+ * with the same sizes (a workspace without a plan for them sets status 7 and
+ * nothing is written); 0 builds it in the call. Needs
  * mb_chunk_workspace_bytes(...) bytes, 256-byte aligned, on the device that is
  * current. Calls that may overlap on the GPU need workspaces of their own.
  * The output does not depend on how the work was scheduled (bit for bit).

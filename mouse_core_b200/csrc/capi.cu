@@ -497,6 +497,10 @@ int chunk_common(mb::ChunkParams* p, mb::ChunkLayout* lay, const int32_t* cu_q, 
   p->key_limit = max_pages * page_size;
   p->sub_tokens = mb::chunk_sub_tokens(p->G);
   p->small_rows = p->G <= 16 ? 16 / p->G * p->G : 0;
+  uint32_t key = 2166136261u;
+  for (int x : {batch, tokens, q_heads, kv_heads, head_dim, page_size, max_pages, sms})
+    key = (key ^ (uint32_t)x) * 16777619u, key ^= key >> 15;
+  p->plan_key = (int)key;
   return MB_OK;
 }
 }  // namespace

@@ -90,10 +90,10 @@ __host__ __device__ constexpr int chunk_tile_cost(bool two_subs, int head_dim) {
 struct ChunkPlanParams {
   const int32_t* cu_q;
   const int32_t* kv_len;
-  int batch, tokens, G, Hkv, tile_tokens, key_limit, sms, max_entries, max_slots, two_subs_cost;
+  int batch, tokens, G, Hkv, tile_tokens, key_limit, sms, max_entries, max_slots, two_subs_cost, plan_key;
   ChunkEntry* entries;
   ChunkSplit* splits;
-  int* head;  // [0] entries, [1] next item, [2] CTAs done, [3] splits, [4] whether a wait ran out
+  int* head;  // [0] entries, [1] next item, [2] CTAs done, [3] splits, [4] whether a wait ran out, [5] the sizes' key
 };
 
 // Key tiles that query tile t of a row (n new tokens, len cached ones) visits.
@@ -239,6 +239,7 @@ __global__ void __launch_bounds__(kChunkPlanThreads) chunk_plan_kernel(const Chu
     if (!fits) report(kDevBadIndex);
     p.head[0] = fits ? total : 0;
     p.head[1] = p.head[2] = p.head[4] = 0;
+    p.head[5] = p.plan_key;
   }
   if (!fits) {
     if (tid == 0) p.head[3] = 0;
@@ -486,7 +487,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       auto wait1 = [&](uint64_t* bar, uint32_t parity) {
         return mbar_wait_or_abort(bar, parity, kDevTimeoutEmpty, &sh->abort);
       };
-      const int n_items = p.head[0] * p.Hkv;
+      const bool planned = p.head[5] == p.plan_key;
+      if (!planned) report(kDevBadIndex);
+      const int n_items = planned ? p.head[0] * p.Hkv : 0;
       // The next piece is taken, and its entry read, when this one's last tiles
       // are loaded: early enough to hide the reads, late enough that a CTA
       // busy with a long piece does not hold on to another.
@@ -637,7 +640,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           if (!(tails >> (issued - 1 - i) & 1)) mbar_drain(&sh->v_full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1);
         // The last CTA resets the counters: the plan serves the next layer too.
         __threadfence();
-        if (atomicAdd(&p.head[2], 1) == (int)gridDim.x - 1) p.head[1] = p.head[2] = 0;
+        if (planned && atomicAdd(&p.head[2], 1) == (int)gridDim.x - 1) p.head[1] = p.head[2] = 0;
       }
     } else if (warp == 1) {
       // --------------------------------------------------------- MMA issue
@@ -1266,7 +1269,7 @@ __global__ void __launch_bounds__(32 * kJoinRows, 4) chunk_join_kernel(const Chu
   constexpr int E = HD / 32;  // output elements per lane
   wait_for_prior_grid();
   const int lane = threadIdx.x & 31;
-  if (p.head[4]) return;
+  if (p.head[4] || p.head[5] != p.plan_key) return;
   const int units = p.head[3] * p.Hkv;
   const size_t step = (size_t)p.Hkv * p.part_rows;
   for (int u = blockIdx.x; u < units; u += gridDim.x) {
@@ -1319,7 +1322,7 @@ size_t chunk_layout(int batch, int tokens, int Hq, int Hkv, int head_dim, int sm
   lay->max_slots = 2 * extra;
   lay->part_rows = (int)std::min<long long>((long long)tokens * G, tile_tokens * G);
   size_t off = 0;
-  lay->head = off;     off = up(off + 5 * sizeof(int));
+  lay->head = off;     off = up(off + 6 * sizeof(int));
   lay->entries = off;  off = up(off + lay->max_entries * sizeof(ChunkEntry));
   lay->splits = off;   off = up(off + extra * ((lay->part_rows + kJoinRows - 1) / kJoinRows) * sizeof(ChunkSplit));
   lay->part_ml = off;  off = up(off + lay->max_slots * Hkv * lay->part_rows * sizeof(float2));
@@ -1341,6 +1344,7 @@ cudaError_t launch_chunk_plan(const ChunkParams& p, const ChunkLayout& lay, uint
   q.key_limit = p.key_limit;
   q.sms = sms;
   q.two_subs_cost = chunk_tile_cost(true, p.head_dim);
+  q.plan_key = p.plan_key;
   q.max_entries = (int)lay.max_entries;
   q.max_slots = (int)lay.max_slots;
   q.entries = reinterpret_cast<ChunkEntry*>(ws + lay.entries);

@@ -26,7 +26,7 @@ enum DeviceStatus : int {
   kDevBadSmem = 4,       // dynamic shared memory base not 1024-byte aligned
   kDevBadPair = 5,       // stored-dS pair index outside the scratch (inconsistent pair offsets)
   kDevTimeoutDrain = 6,  // a CTA's own copies or MMAs did not complete before it exited
-  kDevBadIndex = 7,      // an embedding id outside its table (the token is left zero)
+  kDevBadIndex = 7,      // an index outside its array, or a work list made for other sizes (left out)
 };
 
 // The library is one translation unit (mouse_b200.cu), so the status word is

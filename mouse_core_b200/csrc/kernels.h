@@ -229,6 +229,7 @@ struct ChunkParams {
   int sub_tokens;              // tokens of a 128-query-row sub-tile
   int small_rows;              // query rows that the small tiles' Q box holds (G <= 16)
   float scale_log2;
+  int plan_key;                // of the sizes; a plan made for others is not used
   // the plan and the split tiles' partials (inside the caller's workspace)
   const ChunkEntry* entries;
   const ChunkSplit* splits;

@@ -349,7 +349,8 @@ def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     cached value also of those whose last 128-slot tile holds it. Unused slots
     may hold anything. ``workspace`` (uint8, at least
     ``chunk_workspace_bytes``) is allocated for the call when not given;
-    ``plan_ready`` takes the work list that ``chunk_plan`` left in it."""
+    ``plan_ready`` takes the work list that ``chunk_plan`` left in it for the same
+    sizes (another one is reported as status 7 and writes nothing)."""
     dev = q.get_device() if isinstance(q, torch.Tensor) and q.dtype is BF16 else -1
     if not (_all_on(dev, BF16, k_pool, v_pool) and _all_on(dev, torch.int32, block_table, cu_q, kv_len)):
         _need(q, "q", BF16, contiguous=False)

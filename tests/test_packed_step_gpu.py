@@ -220,8 +220,8 @@ def test_packed_call_without_tokens_and_refusals():
 
 
 @pytest.mark.parametrize("per_row", [False, True])
-@pytest.mark.parametrize("with_head", [False, True])
-def test_grow_rebuild_packed_matches_the_reference_loop(per_row, with_head):
+@pytest.mark.parametrize("with_head,with_hidden", [(False, False), (True, False), (False, True)])
+def test_grow_rebuild_packed_matches_the_reference_loop(per_row, with_head, with_hidden):
     """The grow-then-rebuild loop with packed calls: rebuilt windows beside
     single appended tokens, one-token calls from a graph, emptied rows."""
     dev = _dev()
@@ -239,7 +239,10 @@ def test_grow_rebuild_packed_matches_the_reference_loop(per_row, with_head):
         if ci % 4 == 3:
             ended[:] = ended & per_row
         rb = ended if per_row else bool(ended.any())
-        out, fed = ours.step(hist, ends, ctx, rebuild=rb, head=head)
+        out, fed, *layers = ours.step(hist, ends, ctx, rebuild=rb, head=head, output_hidden_states=with_hidden)
+        if with_hidden:
+            assert len(layers[0]) == 2 and all(t.shape == out.shape for t in layers[0])
+            _close(layers[0][1].float().cpu().numpy(), out.double().cpu().numpy(), ci)  # (no final norm: the identity)
         ref, ref_fed = oracle.step(hist, ends, ctx, rebuild=rb)
         assert fed.tolist() == np.asarray(ref_fed).tolist(), ci
         S = ref.shape[1]
@@ -290,3 +293,34 @@ def test_chunk_attention_wait_timeout_is_reported_and_recovers(head_dim, lens, n
         ref = oatt.cached_decode_attention(q[at:at + m].float().numpy()[None], [rows[0]], [rows[1]], pos,
                                            head_dim ** -0.5)[0]
         assert np.abs(got[at:at + m] - ref).max() < ATOL, b
+
+
+def test_one_plan_serves_every_layer_and_no_other_sizes():
+    """The work list of a step used for several layers' pools and queries; a
+    workspace without one, or with one for other sizes, is reported and leaves
+    the output as it was."""
+    dev = _dev()
+    from mouse_core_b200 import _lib
+    from mouse_core_b200 import kernels as K
+    from tests.test_chunk_gpu import _attention_reference, _check, _paged
+
+    rows = [(6000, 1), (0, 200), (77, 30), (20000, 2)]
+    layers = [_paged(rows, 16, 8, 128, 64, seed=i) for i in range(3)]
+    table, cu, kv_len = layers[0][3:]
+    T = layers[0][0].shape[0]
+    ws = torch.zeros(K.chunk_workspace_bytes(len(rows), T, 16, 8, 128), dtype=torch.uint8, device=dev)
+    out = torch.full((T, 16, 128), 7.0, dtype=torch.bfloat16, device=dev)
+    q, kp, vp = layers[0][:3]
+    K.chunk_attention(q, kp, vp, table, cu, kv_len, 0.1, out=out, workspace=ws, plan_ready=True)
+    assert _lib.device_status() == 7 and bool((out == 7.0).all())
+    K.chunk_plan(cu, kv_len, T, 16, 8, 128, 64, table.shape[1], ws)
+    for q, kp, vp, t, c, n in layers:
+        got = K.chunk_attention(q, kp, vp, t, c, n, 0.1, workspace=ws, plan_ready=True)
+        _check(got, _attention_reference(q, kp, vp, t, c, n, 0.1))
+    assert _lib.device_status() == 0
+    narrow = t[:, :-1].contiguous()  # (the last layer's own table from here on)
+    K.chunk_attention(q, kp, vp, narrow, cu, kv_len, 0.1, out=out, workspace=ws, plan_ready=True)
+    assert _lib.device_status() == 7 and bool((out == 7.0).all())
+    got = K.chunk_attention(q, kp, vp, t, cu, kv_len, 0.1, workspace=ws, plan_ready=True)
+    _check(got, _attention_reference(q, kp, vp, t, cu, kv_len, 0.1))  # the plan is still there
+    assert _lib.device_status() == 0
