@@ -13,7 +13,8 @@
 // n_b G <= 16 is one "small" tile; a longer one is cut into "big" tiles of two
 // sub-tiles of TS = 128 / G tokens (128 query rows) each. (A big tile with one
 // sub-tile's tokens takes its even key tiles as the one and its odd ones as the
-// other, "dual", and the epilogue joins the two.) Every (tile,
+// other, "dual", and the epilogue joins the two: 3 rows of up to 20 query rows over
+// 131000 keys take 147 us, 167 without.) Every (tile,
 // kv-head) is one item over 128-key tiles of the cache; items with many key
 // tiles are split along the keys into pieces when the step has too few items
 // to fill the SMs (chunk_plan_kernel): each piece leaves (O, max, sum) in fp32,
@@ -38,7 +39,19 @@
 //   warps 12-15  epilogue: big tiles' O out of tensor memory, small tiles' join
 //                over the eight warps; the output or the piece's partial
 // Bounds: single tokens are bound by HBM (a 16-row tile needs 64 KB of K/V per
-// 128 keys), chunks by the softmax's exponentials and the tensor pipe.
+// 128 keys); chunks by the chain of a sub-tile, S -> softmax -> P -> O -> next S:
+// at head_dim 128 it takes 3700 cycles for a pair of sub-tiles whose products
+// alone are 2100, at 64 (S issued ahead, but exponentials for half the products)
+// 3650, and a piece costs 3000 more to start and to end.
+// Measured, with the plan (16/8 heads of 128 in 128-token pages, or 32/8 of 64 in
+// 64-token pages; 6.55 TB/s copied and 1677 TFLOP/s multiplied by the library):
+//   256 single tokens over 64..4096 keys           350 us, 6.2 TB/s
+//   128 rows of 0..4 tokens over 128..16380 (64)   119 us, 5.8 TB/s
+//   48 rows, four of them windows of 1024           74 us
+//   48 x 256 tokens over 1024..8192 keys           535 us, 890 TFLOP/s
+//   64 windows of 500..1024 from empty (64)        401 us, 395 TFLOP/s
+//   700 tokens over 60001 keys                     420 us, 820 TFLOP/s
+//   3 rows of 1..5 tokens over 90000..131000 (64)  145 us, 4.7 TB/s
 //
 // Every wait is bounded (common.cuh); the first one that runs out stops its
 // CTA, and no output of an incomplete item is written.
@@ -71,7 +84,8 @@ constexpr int kChunkKeys = 128;      // keys per tile
 constexpr int kChunkSmallRows = 16;  // query rows of a small tile (one mma.sync row block)
 constexpr int kChunkPlanThreads = 1024;
 // Shortest piece: below it a piece's own cost (its queries, its partial, the
-// join) outweighs what another SM gains.
+// join) outweighs what another SM gains. (Long steps take the same at half and
+// twice this; a short one is spared the join's launch, 4 us.)
 // (Costs are in chunk_tile_cost's units: four tiles of the cheaper kind.)
 constexpr int kMinPieceCost = 8;
 // ... and little is gained by pieces shorter than an SM's share of the step, or
@@ -83,6 +97,7 @@ constexpr int kManyItems = 4;  // items per SM
 // What a key tile costs, in units of half a tile of a small piece or of one with
 // a single sub-tile (both bound by the K/V they read): two sub-tiles' softmax
 // takes 1.3 times that at head_dim 128 (64 KB of K/V a tile) and twice at 64.
+// (All alike, 48 rows with four windows among them take 88 us instead of 75.)
 __host__ __device__ constexpr int chunk_tile_cost(bool two_subs, int head_dim) {
   return !two_subs ? 2 : head_dim == 128 ? 3 : 4;
 }
@@ -102,7 +117,8 @@ __device__ __forceinline__ int chunk_key_tiles(int n, int len, int t, bool small
   return max(1, (max(min(len - n + end, key_limit), 0) + kChunkKeys - 1) / kChunkKeys);
 }
 
-// The work list of a step, in one block with a row per thread. Splitting: with
+// The work list of a step, in one block with a row per thread (5 us for 256
+// rows, most of it the launch and the reads). Splitting: with
 // E entries before it, the longest tiles are cut into pieces that cost at most
 // c, c the smallest that leaves at most one wave of CTAs beyond the waves
 // the unsplit items need anyway (so the partials stay few), and not below the
@@ -337,7 +353,6 @@ struct ChunkTile {
   // for P beside S, so that the next S = Q K^T runs under a tile's exponentials;
   // with 128 P overwrites its S.
   static constexpr bool OWN_P = HD == 64;
-  static constexpr int FMA_EXP = HD == 128 ? 3 : 99;  // pairs of exponentials on the FMA pipe: those whose index has these low bits set
   static constexpr uint32_t T_O = 256, T_P = OWN_P ? 384 : 0, P_STEP = OWN_P ? 64 : 128;
 };
 
@@ -391,10 +406,6 @@ struct ChunkRing {
     }
   }
 };
-
-// Masked keys' scores lie below this (-2^90) on the tcgen05 path, finite so that
-// a row without a visible key computes no NaN; real scores stay far above it.
-constexpr float kChunkMasked = -1.2379401e27f;
 
 template <int HD>
 __global__ void __launch_bounds__(kChunkThreads, 1)
@@ -974,8 +985,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         // missed and tiles took twice as long.)
         const bool masked = __any_sync(0xffffffffu, kv0 + kChunkKeys - 1 > hi);
         // Scores of the keys behind the row's last visible one, whatever they
-        // are, become hugely negative; the first pass writes them back for the
-        // second.
+        // are, become -inf; the first pass writes them back for the second.
         auto load = [&](int half, uint32_t(&v)[64]) {
           tmem_ld32(t_s + 64 * half, *reinterpret_cast<uint32_t(*)[32]>(v));
           tmem_ld32(t_s + 64 * half + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
@@ -989,7 +999,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           if (masked) {
             const int last = hi - kv0 - 64 * half;
 #pragma unroll
-            for (int e = 0; e < 64; ++e) v[e] = e <= last ? v[e] : __float_as_uint(2.f * kChunkMasked);
+            for (int e = 0; e < 64; ++e) v[e] = e <= last ? v[e] : __float_as_uint(-INFINITY);
             tmem_st32(t_s + 64 * half, *reinterpret_cast<uint32_t(*)[32]>(v));
             tmem_st32(t_s + 64 * half + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
             tmem_wait_st();
@@ -1007,7 +1017,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         // division uses the same stale maximum, so the result is exact. (A row
         // that sees no key of the tile keeps -inf; a NaN or +inf among the
         // visible scores makes the maximum, and with it the row, NaN.)
-        const float m_tile = mx <= kChunkMasked ? -INFINITY : fmaf(mx, p.scale_log2, mx - mx);
+        const float m_tile = mx == -INFINITY ? mx : fmaf(mx, p.scale_log2, mx - mx);
         const bool grew = !(m_tile <= m_used + 8.f);
         // P's columns (and O) are free once the tile before is consumed.
         if (C::OWN_P) {
@@ -1054,16 +1064,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               float x0, x1;
               ffma2(x0, x1, __uint_as_float(v[32 * c + e]), __uint_as_float(v[32 * c + e + 1]), p.scale_log2,
                     p.scale_log2, neg_mu, neg_mu);
-              // One pair in four takes its 2^x on the FMA pipe (relative error
-              // 1e-4, far below the rounding to bf16): the exponentials' own
-              // unit is what both sub-tiles' warps compete for.
-              float p0, p1;
-              if (((e >> 1) & C::FMA_EXP) == C::FMA_EXP) {
-                exp2_fma2(p0, p1, x0, x1);
-              } else {
-                p0 = fast_exp2(x0);
-                p1 = fast_exp2(x1);
-              }
+              // (Some of them by a polynomial on the FMA pipe gained nothing: one
+              // pair in four 545 us against 545 and 426 against 423 at head_dim 128,
+              // one in eight 425 against 403 at 64.)
+              const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
               const int q = 2 * ((e >> 1) & 3);
               fadd2(ls[q], ls[q + 1], ls[q], ls[q + 1], p0, p1);
               pk[e >> 1] = pack_bf16x2(p0, p1);
@@ -1081,8 +1085,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       }
       if (!ok) break;
       sh->stats[k & 1][hh][0][r] = m_used;
-      // (exp2_fma2 gives 2^-126, not 0, for a masked key: a row that saw none has no weight.)
-      sh->stats[k & 1][hh][1][r] = m_used == -INFINITY ? 0.f : l;
+      sh->stats[k & 1][hh][1][r] = l;
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->stats_full[k & 1][hh]);
       J += wk.n;

@@ -17,6 +17,10 @@
 // thread and scans (tokens, pages) itself, so one launch without a grid barrier does
 // the whole step; the tokens and opened pages of a group are spread over the
 // blocks, each token finding its row by bisection in shared memory.
+// Measured, replayed from a graph: 256 rows of one token 5.4 us, with six windows
+// of 1024 tokens among them 6.0, 4096 rows of 0 to 4 tokens 9.4, 64 rows of 1024
+// to 8192 tokens 7.9; called from Python 11.9 us each, of which the launch is 4
+// and two thirds the host's.
 #include "common.cuh"
 #include "kernels.h"
 
