@@ -14,7 +14,7 @@
 // sub-tiles of TS = 128 / G tokens (128 query rows) each. (A big tile with one
 // sub-tile's tokens takes its even key tiles as the one and its odd ones as the
 // other, "dual", and the epilogue joins the two: 3 rows of up to 20 query rows over
-// 131000 keys take 147 us, 167 without.) Every (tile,
+// 131000 keys take 147 us, and 167 without.) Every (tile,
 // kv-head) is one item over 128-key tiles of the cache; items with many key
 // tiles are split along the keys into pieces when the step has too few items
 // to fill the SMs (chunk_plan_kernel): each piece leaves (O, max, sum) in fp32,
@@ -47,11 +47,11 @@
 // 64-token pages; 6.55 TB/s copied and 1677 TFLOP/s multiplied by the library):
 //   256 single tokens over 64..4096 keys           350 us, 6.2 TB/s
 //   128 rows of 0..4 tokens over 128..16380 (64)   119 us, 5.8 TB/s
-//   48 rows, four of them windows of 1024           74 us
+//   48 rows, four of them windows of 1024           72 us
 //   48 x 256 tokens over 1024..8192 keys           535 us, 890 TFLOP/s
 //   64 windows of 500..1024 from empty (64)        401 us, 395 TFLOP/s
 //   700 tokens over 60001 keys                     420 us, 820 TFLOP/s
-//   3 rows of 1..5 tokens over 90000..131000 (64)  145 us, 4.7 TB/s
+//   3 rows of 1..5 tokens over 90000..131000 (64)  142 us, 4.8 TB/s
 //
 // Every wait is bounded (common.cuh); the first one that runs out stops its
 // CTA, and no output of an incomplete item is written.
@@ -86,26 +86,26 @@ constexpr int kChunkPlanThreads = 1024;
 // Shortest piece: below it a piece's own cost (its queries, its partial, the
 // join) outweighs what another SM gains. (Long steps take the same at half and
 // twice this; a short one is spared the join's launch, 4 us.)
-// (Costs are in chunk_tile_cost's units: four tiles of the cheaper kind.)
-constexpr int kMinPieceCost = 8;
+// (In kChunkTileCost's units: four tiles of the cheapest kind.)
+constexpr int kMinPieceCost = 16;
 // ... and little is gained by pieces shorter than an SM's share of the step, or
 // half of it when there are few items: longest first evens those out. (A step
 // of 800 items took 119 us cut at the share and 131 at half of it; 8 items over
 // 131072 keys 199 and 151.)
 constexpr int kManyItems = 4;  // items per SM
 
-// What a key tile costs, in units of half a tile of a small piece or of one with
-// a single sub-tile (both bound by the K/V they read): two sub-tiles' softmax
-// takes 1.3 times that at head_dim 128 (64 KB of K/V a tile) and twice at 64.
-// (All alike, 48 rows with four windows among them take 88 us instead of 75.)
-__host__ __device__ constexpr int chunk_tile_cost(bool two_subs, int head_dim) {
-  return !two_subs ? 2 : head_dim == 128 ? 3 : 4;
-}
+// What a key tile costs, in quarters of a small piece's, which is bound by its
+// K/V (hd 64: 32 KB in 1440 cycles, hd 128: 64 KB in 2700). One sub-tile alone
+// takes 1825 cycles, a pair 3650. (All alike, 48 rows with four windows among
+// them take 88 us instead of 72; pairs at 8 and 6 quarters and single sub-tiles
+// like small pieces 74, and 3 long rows of hd 64 147 instead of 142.)
+enum ChunkKind { kSmallTile, kOneSub, kTwoSubs };
+constexpr int kChunkTileCost[2][3] = {{4, 6, 10}, {4, 5, 7}};  // head_dim 64, 128
 
 struct ChunkPlanParams {
   const int32_t* cu_q;
   const int32_t* kv_len;
-  int batch, tokens, G, Hkv, tile_tokens, key_limit, sms, max_entries, max_slots, two_subs_cost, plan_key;
+  int batch, tokens, G, Hkv, tile_tokens, key_limit, sms, max_entries, max_slots, plan_key, cost[3];
   ChunkEntry* entries;
   ChunkSplit* splits;
   int* head;  // [0] entries, [1] next item, [2] CTAs done, [3] splits, [4] whether a wait ran out, [5] the sizes' key
@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(kChunkPlanThreads) chunk_plan_kernel(const Chu
   // Row r0 + tid: its tokens, keys and tiles.
   int r0 = -1, n = 0, len = 0, tiles = 0, cu = 0;
   bool small = false;
-  int cost = 2;  // of a key tile
+  int cost = 0;  // of a key tile
   auto load = [&](int at) {
     if (at == r0) return;
     r0 = at;
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(kChunkPlanThreads) chunk_plan_kernel(const Chu
       len = max(p.kv_len[r0 + tid], 0);
       small = n <= kChunkSmallRows / p.G;
       tiles = n <= 0 ? 0 : small ? 1 : (n + p.tile_tokens - 1) / p.tile_tokens;
-      cost = n > p.tile_tokens / 2 ? p.two_subs_cost : 2;
+      cost = p.cost[small ? kSmallTile : n > p.tile_tokens / 2 ? kTwoSubs : kOneSub];
     }
   };
   auto key_tiles = [&](int t) { return chunk_key_tiles(n, len, t, small, p.tile_tokens, p.key_limit); };
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(kChunkPlanThreads) chunk_plan_kernel(const Chu
   };
   // Of the row's longest piece (a row with a split tile counts as c: it has
   // pieces near it); 0 comes first.
-  auto bucket = [&]() { return kBuckets - 1 - min(min(key_tiles(tiles - 1) * cost, c) / 2, kBuckets - 1); };
+  auto bucket = [&]() { return kBuckets - 1 - min(min(key_tiles(tiles - 1) * cost, c) / 4, kBuckets - 1); };
   // 3. Where each piece length starts in the order.
   __syncthreads();
   for (int at = 0; at < p.batch; at += blockDim.x) {
@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(kChunkPlanThreads) chunk_plan_kernel(const Chu
       const int n_ = n_s[r], len_ = len_s[r];
       const bool small_ = n_ <= kChunkSmallRows / p.G;
       const int kt = chunk_key_tiles(n_, len_, t, small_, p.tile_tokens, p.key_limit);
-      const int cost_ = n_ > p.tile_tokens / 2 ? p.two_subs_cost : 2;
+      const int cost_ = p.cost[small_ ? kSmallTile : n_ > p.tile_tokens / 2 ? kTwoSubs : kOneSub];
       const int pieces = pieces_of(kt * cost_);
       // Behind the row's longer tiles t + 1 .. last.
       int first = base_s[r] + last - t;
@@ -1346,7 +1346,7 @@ cudaError_t launch_chunk_plan(const ChunkParams& p, const ChunkLayout& lay, uint
   q.tile_tokens = 2 * p.sub_tokens;
   q.key_limit = p.key_limit;
   q.sms = sms;
-  q.two_subs_cost = chunk_tile_cost(true, p.head_dim);
+  for (int i = 0; i < 3; ++i) q.cost[i] = kChunkTileCost[p.head_dim == 128][i];
   q.plan_key = p.plan_key;
   q.max_entries = (int)lay.max_entries;
   q.max_slots = (int)lay.max_slots;
@@ -1391,8 +1391,8 @@ static cudaError_t launch_chunk(const CUtensorMap& qm, const CUtensorMap& sqm, c
   cfg.numAttrs = after_plan ? 1 : 0;
   e = cudaLaunchKernelEx(&cfg, chunk_attention_kernel<HD>, qm, sqm, km, vm, p);
   // A table whose longest tile costs no more than the shortest piece allowed needs no join.
-  const long long most = ((long long)p.key_limit + kChunkKeys - 1) / kChunkKeys *
-                         chunk_tile_cost(p.tokens > p.sub_tokens, HD);
+  const int kind = p.tokens > p.sub_tokens ? kTwoSubs : p.tokens > kChunkSmallRows / p.G ? kOneSub : kSmallTile;
+  const long long most = ((long long)p.key_limit + kChunkKeys - 1) / kChunkKeys * kChunkTileCost[HD == 128][kind];
   if (e != cudaSuccess || most <= kMinPieceCost) return e;
   cfg.gridDim = dim3(8 * grid);
   cfg.blockDim = dim3(32 * kJoinRows);
