@@ -617,6 +617,7 @@ class PagedDecodeSession:
         ev.record()
         if stale:
             if self._bt_dev.shape[1] != width:
+                self._bt_dev.record_stream(torch.cuda.current_stream(self.device))
                 self._bt_dev = torch.empty((B, width), dtype=torch.int32, device=self.device)
             self._bt_dev.copy_(dev[2 * B + total:].view(B, width))
             pages.dirty = False
@@ -812,6 +813,8 @@ class PagedDecodeSession:
         Hq, Hkv, hd = self.n_heads, self.n_kv_heads, self.head_dim
         need = K.chunk_workspace_bytes(self.B, tokens, Hq, Hkv, hd)
         if self._chunk_workspace.numel() < need:
+            # (Its memory may be from another stream, with this one's last call still on it.)
+            self._chunk_workspace.record_stream(torch.cuda.current_stream(self.device))
             self._chunk_workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
         K.chunk_plan(cu_q, kv_len, tokens, Hq, Hkv, hd, self.page_size, self._bt_dev.shape[1], self._chunk_workspace)
         return True
