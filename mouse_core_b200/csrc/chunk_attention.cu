@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       uint32_t tails = 0;                              // bit i: the tile issued i tiles ago was one of them
       for (int k = 0;; ++k) {
         bool ok = true;
-        ChunkWork wk;
+        ChunkWork wk{};
         // Q: the small buffer of this parity is free once piece k - 2 is done, a
         // sub-tile's (the small pieces' join area) once piece k - 1 is. The
         // second sub-tile's is loaded behind the first K/V tile, whose stage is
