@@ -172,6 +172,7 @@ __global__ void __launch_bounds__(kChunkPlanThreads) chunk_plan_kernel(const Chu
     load(at);
     if (n > 0 && len > p.key_limit) report(kDevBadPage);
     count += tiles;
+    if (count > p.max_entries) continue;  // too many already (below): bounds this loop, too
     for (int t = 0; t < tiles; ++t) sum += key_tiles(t) * cost;
     if (tiles > 0) most = max(most, key_tiles(tiles - 1) * cost);
   }
@@ -185,6 +186,16 @@ __global__ void __launch_bounds__(kChunkPlanThreads) chunk_plan_kernel(const Chu
   }
   __syncthreads();
   const long long E = (long long)warp_add(lane < nw ? (unsigned long long)warp_tot[lane] : 0);
+  // Offsets that overlap can ask for more tiles than the stream holds. Such a
+  // step has no plan; below, no 32-bit count of tiles or pieces can wrap.
+  auto no_plan = [&]() {
+    if (tid == 0) {
+      report(kDevBadIndex);
+      p.head[0] = p.head[1] = p.head[2] = p.head[3] = p.head[4] = 0;
+      p.head[5] = p.plan_key;
+    }
+  };
+  if (E > p.max_entries) return no_plan();
   sum = warp_add(lane < nw ? warp_sum[lane] : 0);
   most = __reduce_max_sync(all, lane < nw ? warp_max[lane] : 0);
   // 2. The piece length c, by bisection.
@@ -250,16 +261,11 @@ __global__ void __launch_bounds__(kChunkPlanThreads) chunk_plan_kernel(const Chu
     total += __reduce_add_sync(all, tot);
     __syncthreads();
   }
-  const bool fits = total <= p.max_entries;  // offsets that overlap can ask for more tiles than the stream holds
+  if (total > p.max_entries) return no_plan();
   if (tid == 0) {
-    if (!fits) report(kDevBadIndex);
-    p.head[0] = fits ? total : 0;
+    p.head[0] = total;
     p.head[1] = p.head[2] = p.head[4] = 0;
     p.head[5] = p.plan_key;
-  }
-  if (!fits) {
-    if (tid == 0) p.head[3] = 0;
-    return;
   }
   // 4. The entries: the group's tiles side by side, each finding its row by
   // bisection.

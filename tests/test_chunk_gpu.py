@@ -476,3 +476,31 @@ def test_what_a_token_sees_decides_whether_its_output_is_a_number(hd, bad):
     sees[-1, 3] = True
     assert bool(torch.isnan(out[sees].float()).all())
     _check(out[~sees], (o[~sees], A[~sees]))
+
+
+@pytest.mark.parametrize("group,T,full", [(2, 2000, 40), (1, 300, 700), (128, 524288, 8192)])
+def test_overlapping_rows_that_ask_for_more_tiles_than_the_stream_holds(group, T, full):
+    """Offsets 0, T, 0, T, ...: every second row asks for the whole stream. The
+    last case asks for 2^31 tiles, which no 32-bit count holds. The step is
+    reported, no entry is written past the workspace, and (the sizes at which
+    queries are worth making) the output stays as it was."""
+    dev = _dev()
+    from mouse_core_b200 import kernels as K
+
+    B = 2 * full - 1
+    cu = torch.tensor([0, T] * full, dtype=torch.int32, device=dev)
+    kv_len = torch.full((B,), 100, dtype=torch.int32, device=dev)
+    need = K.chunk_workspace_bytes(B, T, group, 1, 64)
+    buf = torch.full((need + (1 << 22),), 0xA5, dtype=torch.uint8, device=dev)
+    ws = buf[1 << 21: (1 << 21) + need]
+    K.chunk_plan(cu, kv_len, T, group, 1, 64, 64, 2, ws)
+    torch.cuda.synchronize()
+    assert _status() == 7
+    assert bool((buf[: 1 << 21] == 0xA5).all()) and bool((buf[(1 << 21) + need:] == 0xA5).all())
+    if T > 4096:
+        return
+    pool = torch.zeros(2, 1, 64, 64, dtype=torch.bfloat16, device=dev)
+    table = torch.zeros(B, 2, dtype=torch.int32, device=dev)
+    out = torch.full((T, group, 64), 7.0, dtype=torch.bfloat16, device=dev)
+    K.chunk_attention(torch.zeros_like(out), pool, pool, table, cu, kv_len, 0.1, out=out)
+    assert _status() == 7 and bool((out == 7.0).all())
