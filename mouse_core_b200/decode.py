@@ -202,6 +202,7 @@ class PagedDecodeSession:
         self._new_page_dev = torch.full((self.B,), -1, dtype=torch.int32, device=self.device)
         self._step_args: tuple | None = None  # pointers of the captured graph's metadata views
         self._graph = None
+        self._graph_x = None
         self._graph_key = None
         self._graph_warm = False
         # decode_step's graph: embedding gather + layer stack + norm + head.
@@ -358,6 +359,12 @@ class PagedDecodeSession:
         self._len[dst] = plen
 
     # ------------------------------------------------------------------ pool
+    def _outgrown(self, t: torch.Tensor) -> None:
+        """Call before ``t`` is replaced. Its memory may be from another stream
+        (of the session's creation, or of an earlier call), whose next
+        allocation could take it while this stream still works on it."""
+        t.record_stream(torch.cuda.current_stream(self.device))
+
     def _grow_pool(self, need_free: int) -> None:
         self._device_step_ok = False
         old = self.pages.num_pages
@@ -367,6 +374,7 @@ class PagedDecodeSession:
             src = getattr(self, name)
             dst = torch.zeros(shape, device=self.device, dtype=self.dtype)
             dst[:, :old] = src
+            self._outgrown(src)
             setattr(self, name, dst)
         self.pages.grow_pool(new)
 
@@ -435,6 +443,7 @@ class PagedDecodeSession:
         if bt_changed:
             host[o:o + B * width] = self.pages.table.reshape(-1)
         if self._meta_dev.numel() < n_meta:
+            self._outgrown(self._meta_dev)
             self._meta_dev = torch.empty(max(n_meta, 2 * self._meta_dev.numel()), dtype=torch.int32,
                                          device=self.device)
             self._graph = None  # its captured views point at the old buffer
@@ -450,6 +459,7 @@ class PagedDecodeSession:
         slot_d = dev[B * S + B:2 * B * S + B]
         if bt_changed:
             if self._bt_dev.shape[1] != width:
+                self._outgrown(self._bt_dev)
                 self._bt_dev = torch.empty((B, width), dtype=torch.int32, device=self.device)
             self._bt_dev.copy_(dev[2 * B * S + B:n_meta].view(B, width))
             self.pages.dirty = False
@@ -565,6 +575,8 @@ class PagedDecodeSession:
                 self._graph_warm = True
                 return self._final(self._body(x, q_pos, kv_len, slot, 1, False).view(B, S, D))
             self._graph = None
+            if self._graph_x is not None:
+                self._outgrown(self._graph_x)
             self._graph_x = torch.empty_like(x)
             self._graph_x.copy_(x)
             graph = torch.cuda.CUDAGraph()
@@ -617,7 +629,7 @@ class PagedDecodeSession:
         ev.record()
         if stale:
             if self._bt_dev.shape[1] != width:
-                self._bt_dev.record_stream(torch.cuda.current_stream(self.device))
+                self._outgrown(self._bt_dev)
                 self._bt_dev = torch.empty((B, width), dtype=torch.int32, device=self.device)
             self._bt_dev.copy_(dev[2 * B + total:].view(B, width))
             pages.dirty = False
@@ -736,6 +748,8 @@ class PagedDecodeSession:
             h = self._body(x, q_pos, kv_len, slot, 1, False)
             return head(self.model.norm(h.view(B, 1, -1))[:, -1])
         self._step_graph = None
+        if self._step_ids is not None:
+            self._outgrown(self._step_ids)
         self._step_ids = torch.empty_like(ids, device=self.device)
         self._step_ids.copy_(ids)
         graph = torch.cuda.CUDAGraph()
@@ -795,6 +809,7 @@ class PagedDecodeSession:
         if split:
             need = K.decode_workspace_bytes(B, Hkv, R, hd, self.cap)
             if self._workspace.numel() < need:
+                self._outgrown(self._workspace)
                 self._workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
                 self._graph = None
                 self._step_graph = None
@@ -803,6 +818,7 @@ class PagedDecodeSession:
             K.decode_plan(kv_len, Hkv, R, hd, self.cap, self._workspace,
                           block_table=self._bt_dev if S == 1 else None, page_size=self.page_size)
         elif self._workspace.numel() < 256:  # prefill chunks keep a tile counter in it
+            self._outgrown(self._workspace)
             self._workspace = torch.empty(256, dtype=torch.uint8, device=self.device)
             self._graph = None
             self._step_graph = None
@@ -813,8 +829,7 @@ class PagedDecodeSession:
         Hq, Hkv, hd = self.n_heads, self.n_kv_heads, self.head_dim
         need = K.chunk_workspace_bytes(self.B, tokens, Hq, Hkv, hd)
         if self._chunk_workspace.numel() < need:
-            # (Its memory may be from another stream, with this one's last call still on it.)
-            self._chunk_workspace.record_stream(torch.cuda.current_stream(self.device))
+            self._outgrown(self._chunk_workspace)
             self._chunk_workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
         K.chunk_plan(cu_q, kv_len, tokens, Hq, Hkv, hd, self.page_size, self._bt_dev.shape[1], self._chunk_workspace)
         return True

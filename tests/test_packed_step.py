@@ -60,3 +60,42 @@ def test_prepare_packed_refuses_lengths_that_do_not_fit(lengths):
         s.prepare_packed(lengths, 4)
     # Nothing was allocated or advanced by a refused call.
     assert s.pages.free_pages == 8 and s._len.tolist() == [0, 5, 64] and s.pages.npages.tolist() == [0, 0, 0]
+
+
+@pytest.fixture
+def recorded(monkeypatch):
+    """Which tensors were put under which stream, and a stream to stand on."""
+    seen = []
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: seen.append((t.data_ptr(), t.numel(), s)),
+                        raising=False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: "side")
+    return seen
+
+
+def test_pools_outgrown_on_another_stream_stay_until_that_stream_is_done(recorded):
+    s = _stub()
+    s.n_kv_heads, s.head_dim = 2, 64
+    s.k_pool = torch.randn(1, 8, 2, 64, 64).bfloat16()
+    s.v_pool = torch.randn(1, 8, 2, 64, 64).bfloat16()
+    old = s.k_pool, s.v_pool
+    s._grow_pool(12)
+    assert s.pages.num_pages >= 12 and s.k_pool.shape[1] == s.v_pool.shape[1] == s.pages.num_pages
+    assert torch.equal(s.k_pool[:, :8], old[0]) and torch.equal(s.v_pool[:, :8], old[1])
+    for t in old:
+        assert (t.data_ptr(), t.numel(), "side") in recorded
+
+
+def test_metadata_outgrown_on_another_stream_stays_until_that_stream_is_done(recorded, monkeypatch):
+    """A padded call that widens the block table and enlarges the metadata buffer."""
+    s = _stub()
+    s._pending_reset = np.zeros(3, dtype=bool)
+    s._staging_ev = [SimpleNamespace(record=lambda: None)] * 2
+    s._stage = lambda n: (torch.empty(n, dtype=torch.int32), 0)
+    s._meta_dev, s._bt_dev = torch.zeros(2, dtype=torch.int32), torch.zeros(3, 2, dtype=torch.int32)
+    s.pages = PageTable(3, 20, 64, 2)
+    s._len = np.zeros(3, dtype=np.int64)
+    old = s._meta_dev, s._bt_dev
+    s.prepare([200, 3, 0], 200)
+    assert s._bt_dev.shape[1] > 2 and s._meta_dev.numel() > 2
+    for t in old:
+        assert (t.data_ptr(), t.numel(), "side") in recorded

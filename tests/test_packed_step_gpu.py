@@ -324,3 +324,36 @@ def test_one_plan_serves_every_layer_and_no_other_sizes():
     got = K.chunk_attention(q, kp, vp, t, cu, kv_len, 0.1, workspace=ws, plan_ready=True)
     _check(got, _attention_reference(q, kp, vp, t, cu, kv_len, 0.1))  # the plan is still there
     assert _lib.device_status() == 0
+
+
+def test_growth_on_a_side_stream_beside_allocations_on_the_session_s_own():
+    """A session made on one stream and stepped on another outgrows its pool
+    and its table there, while the first stream allocates and fills memory of
+    the sizes just given up."""
+    dev = _dev()
+    bb, dec = _model(dev, 128, 4, 2)
+    gen = torch.Generator().manual_seed(8)
+    B, D = 3, 256
+    sess = bb.decode_session(batch_size=B, capacity=64, page_size=64, num_pages=3)
+    oracle = _Rows(dec, B)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    # Work in front of the session's own, so that its copies are still to come
+    # when the other stream allocates.
+    busy = torch.randn(4096, 4096, device=dev)
+    results = []
+    for n in ([40, 3, 60], [500, 1, 1], [1, 900, 40], [1, 1, 1200], [2, 1, 1]):
+        parts = [torch.randn(k, D, generator=gen).bfloat16() for k in n]
+        ref, _ = oracle.step([p.double().numpy() for p in parts])
+        x = torch.cat(parts).to(dev)
+        side.wait_stream(torch.cuda.current_stream())
+        sizes = [sess.k_pool.numel() * 2, sess.v_pool.numel() * 2, sess.block_table.numel() * 4]
+        with torch.cuda.stream(side):
+            for _ in range(4):
+                busy @ busy
+            results.append((sess.forward_packed(embeds=x, lengths=n), ref, n, x))  # (x is the default stream's)
+        fill = [torch.full((k,), 0xFF, dtype=torch.uint8, device=dev) for k in sizes for _ in range(2)]
+        del fill
+    torch.cuda.synchronize()
+    for got, ref, n, _ in results:
+        _close(got.float().cpu().numpy(), ref, n)
