@@ -611,7 +611,14 @@ class PagedDecodeSession:
         if total > pages.free_pages:
             self._grow_pool(total)
         stale = pages.dirty or bool(self._pending_reset.any()) or self._bt_dev.shape[1] != pages.max_pages
-        ids = pages.open_chunks(add)
+        pages.open_chunks(add)
+        # The device's table lacks the new entries until K14 is launched: a
+        # call that fails before has the next one send the whole table. K14
+        # counts the pages a row opens from its lengths, so the ids are the
+        # table's, too (a row may hold pages that a failed call opened).
+        pages.dirty = True
+        ids = pages.columns(-(-self._len // self.page_size), -(-new_len // self.page_size))
+        total = ids.shape[0]
         width = pages.max_pages
         stale = stale or self._bt_dev.shape[1] != width
         n_meta = 2 * B + total + (B * width if stale else 0)
@@ -632,10 +639,10 @@ class PagedDecodeSession:
                 self._outgrown(self._bt_dev)
                 self._bt_dev = torch.empty((B, width), dtype=torch.int32, device=self.device)
             self._bt_dev.copy_(dev[2 * B + total:].view(B, width))
-            pages.dirty = False
-            self._pending_reset[:] = False
         cu_q, q_pos, slot, kv_len, _ = K.chunk_meta(dev[:B], dev[B:2 * B], self._bt_dev, dev[2 * B:2 * B + total],
                                                     self.page_size, tokens)
+        pages.dirty = False
+        self._pending_reset[:] = False
         self._len = new_len
         self._device_step_ok = False  # K8's buffers still hold the step before
         return q_pos, kv_len, slot, cu_q
@@ -649,7 +656,8 @@ class PagedDecodeSession:
         the tuple of per-layer hidden states.
 
         The cache, ``reset_rows`` and ``fork`` are those of ``forward``; calls
-        of both kinds may follow one another in any order. Every GEMM, norm and
+        of both kinds may follow one another in any order, and a call that raises
+        (out of memory, say) leaves the rows as long as they were. Every GEMM, norm and
         attention tile works on real tokens only, so a call that mixes long
         chunks with single tokens costs what its tokens cost, where ``forward``
         costs ``B`` times its longest chunk (two layers of hidden size 1024, 256
@@ -664,10 +672,15 @@ class PagedDecodeSession:
                 raise RuntimeError("forward_packed reads lengths on the host and cannot be captured")
             T = embeds.shape[0]
             x = embeds.to(self.device, self.dtype).contiguous()
+            before = self._len
             q_pos, kv_len, slot, cu_q = self.prepare_packed(lengths, T)
             if T == 0:
                 return (x, tuple(x for _ in range(self.n_layers))) if output_hidden_states else x
-            out = self._body(x, q_pos, kv_len, slot, 0, output_hidden_states, cu_q)
+            try:
+                out = self._body(x, q_pos, kv_len, slot, 0, output_hidden_states, cu_q)
+            except BaseException:
+                self._len = before  # (slots behind a row's length are never read)
+                raise
             if output_hidden_states:
                 h, hiddens = out
                 return self._final(h), tuple(t.to(self.dtype) for t in hiddens)

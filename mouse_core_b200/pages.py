@@ -96,6 +96,15 @@ class PageTable:
         self.npages += add
         return ids
 
+    def columns(self, first: np.ndarray, last: np.ndarray) -> np.ndarray:
+        """The ids in columns ``first[b] .. last[b] - 1`` of every row, row by row."""
+        n = last - first
+        total = int(n.sum())
+        if total == 0:
+            return np.empty(0, dtype=np.int32)
+        starts = first - (np.cumsum(n) - n)
+        return self.table[np.repeat(np.arange(self.B), n), np.arange(total) + np.repeat(starts, n)]
+
     def open_pages(self, rows: np.ndarray) -> np.ndarray:
         """Append one fresh page to each of ``rows`` (distinct, ascending; the
         table must have a free column for each) and return the ids: the same

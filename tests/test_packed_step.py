@@ -99,3 +99,87 @@ def test_metadata_outgrown_on_another_stream_stays_until_that_stream_is_done(rec
     assert s._bt_dev.shape[1] > 2 and s._meta_dev.numel() > 2
     for t in old:
         assert (t.data_ptr(), t.numel(), "side") in recorded
+
+
+def _device_table(table, n, c, free, page):
+    """What K14 does to the device's block table, and the slots it makes."""
+    slots, taken = [], 0
+    for b in range(len(n)):
+        held, total = -(-int(c[b]) // page), -(-int(c[b] + n[b]) // page)
+        for col in range(held, total):
+            if taken < len(free):
+                table[b, col] = free[taken]
+            taken += 1
+        slots += [int(table[b, p // page]) * page + p % page for p in range(int(c[b]), int(c[b] + n[b]))]
+    assert taken <= len(free), "K14 was given too few pages"
+    return slots
+
+
+@pytest.mark.parametrize("fails_in", ["stage", "upload", "K14"])
+@pytest.mark.parametrize("retry", [[70, 1, 1], [3, 130, 0], [0, 0, 70]])
+def test_a_packed_call_that_failed_leaves_the_next_one_right(recorded, monkeypatch, fails_in, retry):
+    """Out of memory between the pages' opening and the K14 launch: the call
+    made again, or another one, gives every token the slot of the host's table,
+    and so does the padded call behind it."""
+    from mouse_core_b200 import decode
+
+    P = 64
+    s = _stub()
+    s._pending_reset = np.zeros(3, dtype=bool)
+    s._staging_ev = [SimpleNamespace(record=lambda: None)] * 2
+    s._meta_dev = torch.zeros(0, dtype=torch.int32)
+    s._bt_dev = torch.full((3, 4), -1, dtype=torch.int32)
+    s.pages = PageTable(3, 30, P, 4)
+    s._len = np.zeros(3, dtype=np.int64)
+    fail = {"stage": False, "upload": False, "K14": False}
+
+    class Upload(torch.Tensor):
+        def to(self, *a, **k):
+            if fail["upload"]:
+                raise torch.OutOfMemoryError("upload")
+            return super().to(*a, **k).as_subclass(torch.Tensor)
+
+    def stage(n):
+        if fail["stage"]:
+            raise torch.OutOfMemoryError("stage")
+        return torch.empty(n, dtype=torch.int32).as_subclass(Upload), 0
+
+    def chunk_meta(n, c, table, free, page, tokens):
+        if fail["K14"]:
+            raise torch.OutOfMemoryError("K14")
+        assert n.sum() == tokens
+        slots = _device_table(table.numpy(), n.numpy(), c.numpy(), free.tolist(), page)
+        return None, None, torch.tensor(slots), n + c, None
+
+    s._stage = stage
+    monkeypatch.setattr(decode.K, "chunk_meta", chunk_meta)
+
+    def check(lengths):
+        before = s._len.copy()
+        _, _, slots, _ = s.prepare_packed(lengths, sum(lengths))
+        rows = np.repeat(np.arange(3), lengths)
+        pos = np.concatenate([np.arange(c, c + n) for c, n in zip(before, lengths)]).astype(np.int64)
+        assert slots.tolist() == s.pages.slots(rows, pos).tolist()
+        for b in range(3):
+            held = -(-int(s._len[b]) // P)
+            assert s._bt_dev[b, :held].tolist() == s.pages.table[b, :held].tolist()
+
+    check([5, 64, 1])
+    fail[fails_in] = True
+    with pytest.raises(torch.OutOfMemoryError):
+        s.prepare_packed([70, 1, 1], 72)
+    fail[fails_in] = False
+    assert s._len.tolist() == [5, 64, 1]
+    check(retry)
+    check([1, 1, 80])
+    # A padded call behind a failed one: its rows' pages reach the device, too.
+    fail[fails_in] = True
+    with pytest.raises(torch.OutOfMemoryError):
+        s.prepare_packed([130, 60, 0], 190)
+    fail[fails_in] = False
+    s.prepare([2, 60, 0], 60)
+    for b in range(3):
+        held = int(s.pages.npages[b])
+        assert s._bt_dev[b, :held].tolist() == s.pages.table[b, :held].tolist()
+    ids = np.concatenate([s.pages.table[b, :int(s.pages.npages[b])] for b in range(3)])
+    assert len(set(ids.tolist())) == ids.size == 30 - s.pages.free_pages

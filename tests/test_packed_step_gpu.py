@@ -357,3 +357,45 @@ def test_growth_on_a_side_stream_beside_allocations_on_the_session_s_own():
     torch.cuda.synchronize()
     for got, ref, n, _ in results:
         _close(got.float().cpu().numpy(), ref, n)
+
+
+def test_a_packed_call_that_raised_can_be_made_again(monkeypatch):
+    """Out of memory before the metadata launch, and in a layer behind the
+    first one's append: the rows keep their lengths, and the same call, another
+    one and a one-token step come out as if nothing had happened."""
+    dev = _dev()
+    from mouse_core_b200 import decode
+
+    bb, dec = _model(dev, 64, 6, 2)
+    gen = torch.Generator().manual_seed(4)
+    B, D = 3, 256
+    sess = bb.decode_session(batch_size=B, capacity=64, page_size=64, num_pages=4)
+    oracle = _Rows(dec, B)
+
+    def run(n, fails_in=None):
+        parts = [torch.randn(k, D, generator=gen).bfloat16() for k in n]
+        x = torch.cat(parts).to(dev)
+        if fails_in:
+            def fail(*a, **k):
+                raise torch.OutOfMemoryError(fails_in)
+
+            before = sess.lengths.tolist()
+            with monkeypatch.context() as m:
+                m.setattr(decode.K, fails_in, fail)
+                with pytest.raises(torch.OutOfMemoryError):
+                    sess.forward_packed(embeds=x, lengths=n)
+            assert sess.lengths.tolist() == before
+            if fails_in == "chunk_meta":  # another call comes first
+                run([1, 0, 2])
+        ref, _ = oracle.step([p.double().numpy() for p in parts])
+        _close(sess.forward_packed(embeds=x, lengths=n).float().cpu().numpy(), ref, (n, fails_in))
+        assert sess.lengths.tolist() == oracle.s.lengths.tolist()
+
+    run([3, 64, 1])
+    run([200, 1, 70], "chunk_meta")
+    run([1, 130, 2], "chunk_attention")
+    run([1, 1, 300], "chunk_plan")
+    run([5, 0, 1])
+    from mouse_core_b200 import _lib
+
+    assert _lib.device_status() == 0
