@@ -194,6 +194,7 @@ class GrowRebuildDecoder:
                                  max_cache=self.max_cache)
             starts[rows] = new
             self.cached_starts[rows] = new
+            self.cached_ends[rows] = new  # empty until the call below has run
             self.rebuild_calls += 1
             self.rows_rebuilt += int(rows.size)
         fed = np.maximum(ends - starts, 0)

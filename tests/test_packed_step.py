@@ -183,3 +183,53 @@ def test_a_packed_call_that_failed_leaves_the_next_one_right(recorded, monkeypat
         assert s._bt_dev[b, :held].tolist() == s.pages.table[b, :held].tolist()
     ids = np.concatenate([s.pages.table[b, :int(s.pages.npages[b])] for b in range(3)])
     assert len(set(ids.tolist())) == ids.size == 30 - s.pages.free_pages
+
+
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("per_row", [True, False])
+def test_a_rebuild_that_failed_is_fed_again(per_row, packed):
+    """The session's call raises after the rows were emptied: the same step made
+    again feeds them their whole windows, and the others what they missed."""
+    from mouse_core_b200.grow_rebuild import GrowRebuildDecoder
+
+    class Session:
+        def __init__(self):
+            self.rows, self.fail = [[], [], []], False
+
+        def reset_rows(self, rows):
+            for b in rows:
+                self.rows[b] = []
+
+        def _feed(self, parts):
+            if self.fail:
+                raise torch.OutOfMemoryError("layers")
+            for row, part in zip(self.rows, parts):
+                row += part
+
+        def forward_packed(self, *, embeds, lengths, output_hidden_states):
+            at = np.cumsum(lengths)
+            self._feed([embeds[a - n:a, 0].tolist() for a, n in zip(at, lengths)])
+            return embeds
+
+        def forward(self, *, embeds, lengths, output_hidden_states=False):
+            S = embeds.shape[1]
+            self._feed([embeds[b, S - n:, 0].tolist() for b, n in enumerate(lengths)])
+            return embeds
+
+    d = object.__new__(GrowRebuildDecoder)
+    d.B, d.max_cache, d.start_cache, d.per_row, d.packed = 3, 20, 8, per_row, packed
+    d.session, d.embed = Session(), lambda ids: ids[..., None].float()
+    d.cached_starts, d.cached_ends = np.zeros(3, dtype=np.int64), np.zeros(3, dtype=np.int64)
+    d.rebuild_calls = d.rows_rebuilt = 0
+    d._stage_ids = lambda ids: torch.from_numpy(ids.copy())
+    hist = np.arange(3 * 40).reshape(3, 40)
+    d.step(hist, [5, 6, 7])
+    for ends in ([18, 9, 9], [25, 11, 10], [27, 31, 11]):  # row 0, then row 1 outgrow the cache
+        d.session.fail = True
+        with pytest.raises(torch.OutOfMemoryError):
+            d.step(hist, ends)
+        d.session.fail = False
+        d.step(hist, ends)
+        for b in range(3):
+            assert d.session.rows[b] == hist[b, d.cached_starts[b]:ends[b]].tolist(), (b, ends)
+    assert d.rebuild_calls >= 2
