@@ -241,7 +241,9 @@ int mb_decode_step_meta(int batch, int max_pages, int page_size, const int32_t* 
  *                         entries behind the last row's tokens get 0 and -1
  * Negative lengths count as 0. A step that needs more pages than n_free or
  * max_pages hold (status 3) or more than `tokens` tokens (status 7) writes
- * what fits: tokens without a page get slot -1. All int32, device memory.
+ * what fits: tokens without a page get slot -1. So does, with status 3, a token
+ * whose page is missing in the table (a negative entry, or a cached length past
+ * max_pages) or whose slot passes 32 bits. All int32, device memory.
  * ------------------------------------------------------------------- */
 int mb_chunk_meta(const int32_t* lengths, const int32_t* kv_len, int batch, int32_t* block_table, int max_pages,
                   int page_size, const int32_t* free_pages, int n_free, int tokens, int32_t* cu_q,

@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(kChunkMetaThreads) chunk_meta_kernel(const Chu
         p.new_len[r0 + r] = add_capped(c[i], n[i]);
         // More tokens or pages than the caller gave room for: what fits is done.
         if (en > p.tokens) report(kDevBadIndex);
-        if (eo > p.n_free || (o[i] > 0 && pages_of(c[i], P) + o[i] > p.max_pages)) report(kDevBadPage);
+        if (eo > p.n_free || (n[i] > 0 && pages_of(add_capped(c[i], n[i]), P) > p.max_pages)) report(kDevBadPage);
       }
     }
     if (mine && r0 == 0 && tid == 0) p.cu_q[0] = p.cu_pages[0] = 0;
@@ -145,8 +145,10 @@ __global__ void __launch_bounds__(kChunkMetaThreads) chunk_meta_kernel(const Chu
           id = p.free_pages[cup[r] + (col - held)];
       }
       const long long slot = (long long)id * P + pos % P;
+      const bool held_by_page = id >= 0 && slot <= 0x7fffffffll;
+      if (!held_by_page) report(kDevBadPage);
       p.q_pos[x] = pos;
-      p.slot[x] = id >= 0 && slot <= 0x7fffffffll ? (int)slot : -1;
+      p.slot[x] = held_by_page ? (int)slot : -1;
     }
     __syncthreads();  // the arrays are overwritten by the next group
   }

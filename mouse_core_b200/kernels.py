@@ -289,8 +289,9 @@ def chunk_meta(lengths: torch.Tensor, kv_len: torch.Tensor, block_table: torch.T
     position and cache slot (0 and -1 behind the last row's tokens), the new
     lengths, and the pages opened before each row (``cu_pages[B]``: pages taken
     from ``free_pages``). A step that does not fit is reported through
-    ``_lib.device_status`` (3: out of pages or table columns, 7: out of
-    tokens) and its tokens without a page get slot -1."""
+    ``_lib.device_status`` (3: out of pages or table columns, or a cached page
+    missing in the table, 7: out of tokens) and its tokens without a page get
+    slot -1."""
     dev = lengths.get_device() if isinstance(lengths, torch.Tensor) else -1
     if not _all_on(dev, torch.int32, lengths, kv_len, block_table, free_pages):
         _need(lengths, "lengths", torch.int32)

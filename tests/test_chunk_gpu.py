@@ -123,6 +123,22 @@ def test_chunk_meta_reports_a_step_that_does_not_fit():
     _check_meta(n, c, 64, table, free, 0, status=7)
 
 
+def test_chunk_meta_reports_every_token_without_a_page():
+    """Also where the step itself opens none: a cached length past the table,
+    a table entry without a page, and a page whose slots pass 32 bits."""
+    free = np.array([7, 8], np.int32)
+    table = np.array([[5, 6], [3, -1], [1 << 26, 4]], np.int32)
+    _check_meta([1, 0, 0], [190, 10, 1], 64, table, free, 1, status=3)
+    _check_meta([0, 1, 1], [300, 100, 0], 64, table, free, 2, status=3)
+    _check_meta([1, 0, 0], [10, 0, 300], 64, table, free, 1)  # idle rows are nobody's tokens
+    dev = _dev()
+    from mouse_core_b200 import kernels as K
+
+    args = [torch.tensor(x, dtype=torch.int32, device=dev) for x in ([0, 0, 2], [0, 0, 1], table, free)]
+    got = K.chunk_meta(*args, 64, 2)
+    assert _status() == 3 and got[2].tolist() == [-1, -1] and got[1].tolist() == [1, 2]
+
+
 def test_chunk_meta_refuses_bad_arguments():
     dev = _dev()
     from mouse_core_b200 import kernels as K
