@@ -265,8 +265,13 @@ int mb_chunk_meta(const int32_t* lengths, const int32_t* kv_len, int batch, int3
  * past the table are left out). Offsets must not decrease: a decreasing pair
  * is an empty row, and rows that overlap write the same entries of out in no
  * order, or set status 7 and write nothing when they ask for more tiles than
- * the stream holds. A NaN in a cached key makes NaN of the tokens that see it;
- * one in a cached value also of those whose last 128-slot tile holds it.
+ * the stream holds. A NaN in a cached key makes NaN of the tokens that see it.
+ * A NaN or an infinity in a cached value leaves those no finite number, either,
+ * and may make NaN of tokens before it in the row's chunk: 128 / (q_heads /
+ * kv_heads) consecutive tokens, counted from the chunk's first, are one tile;
+ * its last token's position p makes the tile read the row's values up to slot
+ * p / 128 * 128 + 127, and the weights of its other tokens there are 0 (0 * NaN is
+ * NaN). Other tiles and rows are not reached.
  *
  * mb_chunk_plan builds the step's work list in `workspace` from cu_q and
  * kv_len alone, so one plan serves every layer of a step: pass plan_ready = 1

@@ -346,9 +346,13 @@ def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     layer, the new tokens' K/V already appended); block_table ``[B, max_pages]``,
     cu_q ``[B + 1]``, kv_len ``[B]`` int32. Returns ``out [T, Hq, hd]``; tokens
     behind ``cu_q[B]`` are left as they were, and a token with no visible slot
-    gets 0. A NaN in a cached key makes NaN of the tokens that see it; one in a
-    cached value also of those whose last 128-slot tile holds it. Unused slots
-    may hold anything. ``workspace`` (uint8, at least
+    gets 0. A NaN in a cached key makes NaN of the tokens that see it. A NaN or
+    an infinity in a cached value leaves those no finite number, either, and may
+    make NaN of earlier tokens of the row's chunk: ``128 // (Hq // Hkv)``
+    consecutive tokens, counted from the chunk's first, are one tile, which
+    reads the row's values up to the end of the 128 slots that its last token
+    lies in; weights behind a token are 0, and 0 * NaN is NaN. Other tiles and rows
+    are not reached. Unused slots may hold anything. ``workspace`` (uint8, at least
     ``chunk_workspace_bytes``) is allocated for the call when not given;
     ``plan_ready`` takes the work list that ``chunk_plan`` left in it for the same
     sizes (another one is reported as status 7 and writes nothing)."""

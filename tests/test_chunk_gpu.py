@@ -520,3 +520,42 @@ def test_overlapping_rows_that_ask_for_more_tiles_than_the_stream_holds(group, T
     out = torch.full((T, group, 64), 7.0, dtype=torch.bfloat16, device=dev)
     K.chunk_attention(torch.zeros_like(out), pool, pool, table, cu, kv_len, 0.1, out=out)
     assert _status() == 7 and bool((out == 7.0).all())
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("group", [1, 2, 4])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_which_tokens_a_bad_value_reaches(hd, group, bad):
+    """One NaN or infinity in a cached value: the tokens that see it have no
+    finite output in its element, earlier tokens of a tile that reads as far
+    may have none, and every other token is as exact as without it. (A tile is
+    128 / group tokens of the chunk and reads up to the end of the 128 slots of
+    its last token.)"""
+    _dev()
+    from mouse_core_b200 import kernels as K
+
+    # (cached, new, slot of the bad value): inside the prefix, among the new tokens of small, single and
+    # paired tiles that straddle a multiple of 128, of split rows, and in nobody's tile but its own.
+    rows = [(700, 1, 90), (124, 3, 126), (126, 3, 128), (100, 40, 135), (100, 128, 200), (50, 300, 320),
+            (0, 500, 100), (0, 500, 127), (20000, 2, 20001), (15000, 100, 15090), (300, 60, None), (1000, 1, None)]
+    q, kp, vp, table, cu, kv_len = _paged([r[:2] for r in rows], 2 * group, 2, hd, 64, seed=hd + group)
+    clean = vp.clone()
+    sees = torch.zeros(q.shape[0], dtype=torch.bool, device="cuda")
+    may = sees.clone()
+    ts = 128 // group
+    for b, (c, n, at) in enumerate(rows):
+        if at is None:
+            continue
+        vp[table[b, at // 64], :, at % 64, 1] = bad
+        for i in range(n):
+            last = c + min(n, (i // ts + 1) * ts) - 1
+            sees[int(cu[b]) + i] = c + i >= at
+            may[int(cu[b]) + i] = last >= at // 128 * 128
+    assert bool((may | ~sees).all()) and bool((may & ~sees).any()) and bool((~may).any())
+    out = K.chunk_attention(q, kp, vp, table, cu, kv_len, 0.1)
+    assert _status() == 0
+    assert not bool(torch.isfinite(out[sees][:, :, 1].float()).any())
+    o, A = _attention_reference(q, kp, clean, table, cu, kv_len, 0.1)
+    _check(out[~may], (o[~may], A[~may]))
+    others = [e for e in range(hd) if e != 1]
+    _check(out[:, :, others], (o[:, :, others], A[:, :, others]))
