@@ -54,7 +54,9 @@
 //   3 rows of 1..5 tokens over 90000..131000 (64)  142 us, 4.8 TB/s
 //
 // Every wait is bounded (common.cuh); the first one that runs out stops its
-// CTA, and no output of an incomplete item is written.
+// CTA. A query row's output (or partial) is written only when the row is done,
+// so every element of out is then the result or as it was; that of another row
+// of the same item may be either. Split tiles are not joined.
 #include "common.cuh"
 #include "kernels.h"
 #include "tcgen05.cuh"

@@ -399,3 +399,34 @@ def test_a_packed_call_that_raised_can_be_made_again(monkeypatch):
     from mouse_core_b200 import _lib
 
     assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("limit", [0, 2000, 20000])
+def test_after_a_timeout_an_output_is_the_result_or_as_it_was(head_dim, limit):
+    """Waits of a few cycles run out somewhere in a step of single tokens,
+    chunks of one and two sub-tiles and split rows. Nothing half done is
+    written, and the same call is exact afterwards."""
+    _dev()
+    from mouse_core_b200 import _lib
+    from mouse_core_b200 import kernels as K
+    from tests.test_chunk_gpu import TOL, _attention_reference, _check, _paged
+
+    rows = [(3000, 1), (900, 300), (0, 129), (40, 20), (12000, 2), (700, 1), (9000, 100)] * 3
+    args = (*_paged(rows, 8, 4, head_dim, 64, seed=head_dim), 0.1)
+    o, A = ref = _attention_reference(*args)
+    assert _lib.device_status() == 0
+    try:
+        _lib.set_wait_limit(limit)
+        for _ in range(3):
+            out = torch.full_like(args[0], 7.0)
+            K.chunk_attention(*args, out=out)
+            torch.cuda.synchronize()
+            assert _lib.device_status() in (0, 1, 2, 6)
+            right = (out.double() - o).abs() <= TOL * (A + o.abs())
+            assert bool((right | (out == 7.0)).all())
+    finally:
+        _lib.set_wait_limit(None)
+    out = K.chunk_attention(*args)
+    assert _lib.device_status() == 0
+    _check(out, ref)
