@@ -559,3 +559,42 @@ def test_which_tokens_a_bad_value_reaches(hd, group, bad):
     _check(out[~may], (o[~may], A[~may]))
     others = [e for e in range(hd) if e != 1]
     _check(out[:, :, others], (o[:, :, others], A[:, :, others]))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_scores_in_the_hundreds(hd):
+    """Scores of several hundred, where what fp32 holds of them counts.
+
+    Tolerance. With S the largest sum |scale q_d k_d| over a token's visible keys
+    (64 bits): the fp32 sum of hd exact products is off by at most hd 2^-23 S
+    (each of its additions may truncate); scale, log2(e) and their product are
+    rounded to fp32, as are the scaled score, the maximum and their difference:
+    6 x 2^-24 S. So a weight is off by a factor of at most exp(d), d =
+    (2 hd + 6) 2^-24 S, and a quotient of sums of weights by exp(2 d): 2.2 d (A +
+    |o|) on top of the module's bound, as long as d is below 0.05."""
+    _dev()
+    from mouse_core_b200 import kernels as K
+
+    scale = hd ** -0.5
+    rows = [(900, 1), (300, 200), (0, 70), (2300, 3), (30000, 1), (9000, 100)]
+    q, kp, vp, table, cu, kv_len = _paged(rows, 8, 4, hd, 64, seed=31, spread=10.0)
+    S = torch.zeros(*q.shape[:2], 1, dtype=torch.float64, device="cuda")
+    most = 0.0
+    for b, (c, n) in enumerate(rows):
+        ids = table[b, : -(-(c + n) // 64)].long()
+        k = kp[ids].transpose(0, 1).flatten(1, 2)[:, : c + n].double()
+        at = slice(int(cu[b]), int(cu[b]) + n)
+        qb = q[at].double().unflatten(1, (4, 2))
+        seen = torch.arange(c + n, device="cuda") <= torch.arange(c, c + n, device="cuda")[:, None]
+        s = torch.einsum("thgd,hkd->thgk", qb, k).masked_fill_(~seen[:, None, None], 0.0)
+        most = max(most, s.abs().max().item() * scale)
+        s = torch.einsum("thgd,hkd->thgk", qb.abs(), k.abs()).masked_fill_(~seen[:, None, None], 0.0)
+        S[at] = (s.amax(-1) * scale).flatten(1)[:, :, None]
+    assert 300 < most < 1000
+    d = (2 * hd + 6) * 2.0 ** -24 * S
+    assert d.max().item() < 0.05
+    out = K.chunk_attention(q, kp, vp, table, cu, kv_len, scale)
+    assert _status() == 0
+    o, A = _attention_reference(q, kp, vp, table, cu, kv_len, scale)
+    assert bool(torch.isfinite(out.float()).all())
+    assert bool(((out.double() - o).abs() <= (TOL + 2.2 * d) * (A + o.abs()) + 1e-30).all())
