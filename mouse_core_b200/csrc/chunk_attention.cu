@@ -110,7 +110,7 @@ struct ChunkPlanParams {
   int batch, tokens, G, Hkv, tile_tokens, key_limit, sms, max_entries, max_slots, plan_key, cost[3];
   ChunkEntry* entries;
   ChunkSplit* splits;
-  int* head;  // [0] entries, [1] next item, [2] CTAs done, [3] splits, [4] whether a wait ran out, [5] the sizes' key
+  int* head;  // [0] entries, [1] next item, [2] CTAs done, [3] splits, [4] CTAs whose wait ran out, [5] the sizes' key
 };
 
 // Key tiles that query tile t of a row (n new tokens, len cached ones) visits.
@@ -657,9 +657,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         drain_ring(sh->v_tail, C::STAGES, tails_issued);
         for (int i = max(issued - C::STAGES, 0); i < issued; ++i)
           if (!(tails >> (issued - 1 - i) & 1)) mbar_drain(&sh->v_full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1);
-        // The last CTA resets the counters: the plan serves the next layer too.
-        __threadfence();
-        if (planned && atomicAdd(&p.head[2], 1) == (int)gridDim.x - 1) p.head[1] = p.head[2] = 0;
       }
     } else if (warp == 1) {
       // --------------------------------------------------------- MMA issue
@@ -1270,7 +1267,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     __syncwarp();
     tmem_dealloc(tbase, 512);
   }
-  if (threadIdx.x == 0 && *reinterpret_cast<volatile int*>(&sh->abort)) p.head[4] = 1;  // nothing to join until the next plan
+  // The last CTA resets the counters, so that the plan serves the next layer
+  // too, and notes whether there is anything to join: not if a wait ran out in
+  // any CTA (counted in the upper half).
+  if (threadIdx.x == 0 && p.head[5] == p.plan_key) {
+    const int gave_up = *reinterpret_cast<volatile int*>(&sh->abort) != 0;
+    __threadfence();
+    const int done = atomicAdd(&p.head[2], 1 + (gave_up << 16)) + (gave_up << 16);
+    if ((done & 0xffff) == (int)gridDim.x - 1) {
+      p.head[1] = p.head[2] = 0;
+      p.head[4] = done >> 16;
+    }
+  }
 }
 
 // out of the split tiles: over a row's pieces, in their order, M = max m,

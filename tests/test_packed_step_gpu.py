@@ -430,3 +430,26 @@ def test_after_a_timeout_an_output_is_the_result_or_as_it_was(head_dim, limit):
     out = K.chunk_attention(*args)
     assert _lib.device_status() == 0
     _check(out, ref)
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_a_plan_serves_the_call_behind_one_that_timed_out(head_dim):
+    """Split rows are joined again by the next call on the same work list."""
+    dev = _dev()
+    from mouse_core_b200 import _lib
+    from mouse_core_b200 import kernels as K
+    from tests.test_chunk_gpu import _attention_reference, _check, _paged
+
+    rows = [(20000, 1), (300, 90), (9000, 100), (50, 1)]
+    args = (*_paged(rows, 8, 4, head_dim, 64, seed=3), 0.1)
+    q, _, _, table, cu, kv_len, _ = args
+    ref = _attention_reference(*args)
+    ws = torch.zeros(K.chunk_workspace_bytes(len(rows), q.shape[0], 8, 4, head_dim), dtype=torch.uint8, device=dev)
+    K.chunk_plan(cu, kv_len, q.shape[0], 8, 4, head_dim, 64, table.shape[1], ws)
+    run = lambda: K.chunk_attention(*args, out=torch.full_like(q, 7.0), workspace=ws, plan_ready=True)
+    _check(run(), ref)
+    _timed_out_launches(run)
+    for _ in range(2):
+        out = run()
+        assert _lib.device_status() == 0
+        _check(out, ref)
