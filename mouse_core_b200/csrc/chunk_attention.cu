@@ -110,7 +110,9 @@ struct ChunkPlanParams {
   int batch, tokens, G, Hkv, tile_tokens, key_limit, sms, max_entries, max_slots, plan_key, cost[3];
   ChunkEntry* entries;
   ChunkSplit* splits;
-  int* head;  // [0] entries, [1] next item, [2] CTAs done, [3] splits, [4] CTAs whose wait ran out, [5] the sizes' key
+  // [0] entries, [1] next item, [2] CTAs done, [3] splits, [4] whether a wait ran out, [5] the sizes' key, [6] join
+  // blocks that saw [4]
+  int* head;
 };
 
 // Key tiles that query tile t of a row (n new tokens, len cached ones) visits.
@@ -193,7 +195,7 @@ __global__ void __launch_bounds__(kChunkPlanThreads) chunk_plan_kernel(const Chu
   auto no_plan = [&]() {
     if (tid == 0) {
       report(kDevBadIndex);
-      p.head[0] = p.head[1] = p.head[2] = p.head[3] = p.head[4] = 0;
+      p.head[0] = p.head[1] = p.head[2] = p.head[3] = p.head[4] = p.head[6] = 0;
       p.head[5] = p.plan_key;
     }
   };
@@ -266,7 +268,7 @@ __global__ void __launch_bounds__(kChunkPlanThreads) chunk_plan_kernel(const Chu
   if (total > p.max_entries) return no_plan();
   if (tid == 0) {
     p.head[0] = total;
-    p.head[1] = p.head[2] = p.head[4] = 0;
+    p.head[1] = p.head[2] = p.head[4] = p.head[6] = 0;
     p.head[5] = p.plan_key;
   }
   // 4. The entries: the group's tiles side by side, each finding its row by
@@ -657,6 +659,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         drain_ring(sh->v_tail, C::STAGES, tails_issued);
         for (int i = max(issued - C::STAGES, 0); i < issued; ++i)
           if (!(tails >> (issued - 1 - i) & 1)) mbar_drain(&sh->v_full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1);
+        // The last CTA resets the counters: the plan serves the next layer too.
+        __threadfence();
+        if (planned && atomicAdd(&p.head[2], 1) == (int)gridDim.x - 1) p.head[1] = p.head[2] = 0;
       }
     } else if (warp == 1) {
       // --------------------------------------------------------- MMA issue
@@ -1267,18 +1272,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     __syncwarp();
     tmem_dealloc(tbase, 512);
   }
-  // The last CTA resets the counters, so that the plan serves the next layer
-  // too, and notes whether there is anything to join: not if a wait ran out in
-  // any CTA (counted in the upper half).
-  if (threadIdx.x == 0 && p.head[5] == p.plan_key) {
-    const int gave_up = *reinterpret_cast<volatile int*>(&sh->abort) != 0;
-    __threadfence();
-    const int done = atomicAdd(&p.head[2], 1 + (gave_up << 16)) + (gave_up << 16);
-    if ((done & 0xffff) == (int)gridDim.x - 1) {
-      p.head[1] = p.head[2] = 0;
-      p.head[4] = done >> 16;
-    }
-  }
+  if (threadIdx.x == 0 && *reinterpret_cast<volatile int*>(&sh->abort)) p.head[4] = 1;  // nothing to join
 }
 
 // out of the split tiles: over a row's pieces, in their order, M = max m,
@@ -1288,7 +1282,14 @@ __global__ void __launch_bounds__(32 * kJoinRows, 4) chunk_join_kernel(const Chu
   constexpr int E = HD / 32;  // output elements per lane
   wait_for_prior_grid();
   const int lane = threadIdx.x & 31;
-  if (p.head[4] || p.head[5] != p.plan_key) return;
+  if (p.head[5] != p.plan_key) return;
+  if (p.head[4]) {
+    // A wait ran out. The last block takes the mark back, once every thread of
+    // the grid has read it: the next launch on this plan is joined again.
+    __syncthreads();
+    if (threadIdx.x == 0 && atomicAdd(&p.head[6], 1) == (int)gridDim.x - 1) p.head[4] = p.head[6] = 0;
+    return;
+  }
   const int units = p.head[3] * p.Hkv;
   const size_t step = (size_t)p.Hkv * p.part_rows;
   for (int u = blockIdx.x; u < units; u += gridDim.x) {
@@ -1341,7 +1342,7 @@ size_t chunk_layout(int batch, int tokens, int Hq, int Hkv, int head_dim, int sm
   lay->max_slots = 2 * extra;
   lay->part_rows = (int)std::min<long long>((long long)tokens * G, tile_tokens * G);
   size_t off = 0;
-  lay->head = off;     off = up(off + 6 * sizeof(int));
+  lay->head = off;     off = up(off + 7 * sizeof(int));
   lay->entries = off;  off = up(off + lay->max_entries * sizeof(ChunkEntry));
   lay->splits = off;   off = up(off + extra * ((lay->part_rows + kJoinRows - 1) / kJoinRows) * sizeof(ChunkSplit));
   lay->part_ml = off;  off = up(off + lay->max_slots * Hkv * lay->part_rows * sizeof(float2));
