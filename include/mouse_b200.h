@@ -262,8 +262,9 @@ int mb_chunk_meta(const int32_t* lengths, const int32_t* kv_len, int batch, int3
  * of 8; scale > 0. Slots of a page behind the row's last token are not read
  * as values (they may hold NaN). A page id outside the pool reads as zeros
  * and sets status 3, as does a kv_len beyond max_pages * page_size (the keys
- * past the table are left out). Offsets must not decrease: a decreasing pair
- * is an empty row, and rows that overlap write the same entries of out in no
+ * past the table are left out). Rows that reach past `tokens` set status 7 and
+ * get what fits, as mb_chunk_meta writes it: their tokens before the end, at
+ * their positions. Offsets must not decrease: a decreasing pair is an empty row, and rows that overlap write the same entries of out in no
  * order, or set status 7 and write nothing when they ask for more tiles than
  * the stream holds. A NaN in a cached key makes NaN of the tokens that see it.
  * A NaN or an infinity in a cached value leaves those no finite number, either,
@@ -275,8 +276,9 @@ int mb_chunk_meta(const int32_t* lengths, const int32_t* kv_len, int batch, int3
  *
  * mb_chunk_plan builds the step's work list in `workspace` from cu_q and
  * kv_len alone, so one plan serves every layer of a step: pass plan_ready = 1
- * with the same sizes (a workspace without a plan for them sets status 7 and
- * nothing is written); 0 builds it in the call. Needs
+ * with the same sizes and the same lengths in both (a workspace without a plan
+ * for these sizes sets status 7 and nothing is written); 0 builds it in the
+ * call. Needs
  * mb_chunk_workspace_bytes(...) bytes, 256-byte aligned, on the device that is
  * current. Calls that may overlap on the GPU need workspaces of their own.
  * The output does not depend on how the work was scheduled (bit for bit).

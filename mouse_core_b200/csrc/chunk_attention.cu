@@ -151,8 +151,11 @@ __global__ void __launch_bounds__(kChunkPlanThreads) chunk_plan_kernel(const Chu
     n = len = tiles = 0;
     if (r0 + tid < p.batch) {
       cu = min(max(p.cu_q[r0 + tid], 0), p.tokens);
-      n = min(max(p.cu_q[r0 + tid + 1], cu), p.tokens) - cu;
-      len = max(p.kv_len[r0 + tid], 0);
+      const int end = max(p.cu_q[r0 + tid + 1], cu);
+      n = min(end, p.tokens) - cu;
+      // Tokens behind the stream's end are left out, and with them the row's
+      // last keys, which only they see (none may be left: len <= 0).
+      len = max(p.kv_len[r0 + tid], 0) - (end - cu - n);
       small = n <= kChunkSmallRows / p.G;
       tiles = n <= 0 ? 0 : small ? 1 : (n + p.tile_tokens - 1) / p.tile_tokens;
       cost = p.cost[small ? kSmallTile : n > p.tile_tokens / 2 ? kTwoSubs : kOneSub];
@@ -175,6 +178,7 @@ __global__ void __launch_bounds__(kChunkPlanThreads) chunk_plan_kernel(const Chu
   for (int at = 0; at < p.batch; at += blockDim.x) {
     load(at);
     if (n > 0 && len > p.key_limit) report(kDevBadPage);
+    if (r0 + tid < p.batch && p.cu_q[r0 + tid + 1] > p.tokens) report(kDevBadIndex);
     count += tiles;
     if (count > p.max_entries) continue;  // too many already (below): bounds this loop, too
     for (int t = 0; t < tiles; ++t) sum += key_tiles(t) * cost;
@@ -331,7 +335,7 @@ __global__ void __launch_bounds__(kChunkPlanThreads) chunk_plan_kernel(const Chu
         const int k = (kt - k0) / (pieces - i);  // even pieces
         ChunkEntry out;
         out.a = make_int4(row0 + r, cu_s[r] + q0, ntok, len_ - n_ + q0);
-        out.b = make_int4(min(len_, p.key_limit), k0, k, slot);
+        out.b = make_int4(min(max(len_, 0), p.key_limit), k0, k, slot);
         out.c = make_int4(pieces, i, small_, 0);
         p.entries[first + i] = out;
         k0 += k;

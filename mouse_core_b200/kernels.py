@@ -346,16 +346,19 @@ def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     layer, the new tokens' K/V already appended); block_table ``[B, max_pages]``,
     cu_q ``[B + 1]``, kv_len ``[B]`` int32. Returns ``out [T, Hq, hd]``; tokens
     behind ``cu_q[B]`` are left as they were, and a token with no visible slot
-    gets 0. A NaN in a cached key makes NaN of the tokens that see it. A NaN or
+    gets 0. Rows that reach past ``T`` get what fits, at its positions, and set
+    status 7. A NaN in a cached key makes NaN of the tokens that see it. A NaN or
     an infinity in a cached value leaves those no finite number, either, and may
     make NaN of earlier tokens of the row's chunk: ``128 // (Hq // Hkv)``
     consecutive tokens, counted from the chunk's first, are one tile, which
     reads the row's values up to the end of the 128 slots that its last token
-    lies in; weights behind a token are 0, and 0 * NaN is NaN. Other tiles and rows
-    are not reached. Unused slots may hold anything. ``workspace`` (uint8, at least
-    ``chunk_workspace_bytes``) is allocated for the call when not given;
-    ``plan_ready`` takes the work list that ``chunk_plan`` left in it for the same
-    sizes (another one is reported as status 7 and writes nothing)."""
+    lies in; weights behind a token are 0, and 0 * NaN is NaN. Other tiles and
+    rows are not reached. Unused slots may hold anything.
+
+    ``workspace`` (uint8, at least ``chunk_workspace_bytes``) is allocated for
+    the call when not given; ``plan_ready`` takes the work list that
+    ``chunk_plan`` left in it for the same sizes, ``cu_q`` and ``kv_len`` (one for
+    other sizes is reported as status 7 and writes nothing)."""
     dev = q.get_device() if isinstance(q, torch.Tensor) and q.dtype is BF16 else -1
     if not (_all_on(dev, BF16, k_pool, v_pool) and _all_on(dev, torch.int32, block_table, cu_q, kv_len)):
         _need(q, "q", BF16, contiguous=False)

@@ -598,3 +598,50 @@ def test_scores_in_the_hundreds(hd):
     o, A = _attention_reference(q, kp, vp, table, cu, kv_len, scale)
     assert bool(torch.isfinite(out.float()).all())
     assert bool(((out.double() - o).abs() <= (TOL + 2.2 * d) * (A + o.abs()) + 1e-30).all())
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("room", [0, 1, 3, 20, 100, 200, 333])
+def test_rows_that_reach_past_the_stream_get_what_fits(hd, room):
+    """The stream ends inside a row, or before it: the tokens that fit are those
+    of the whole step, at their own positions, and the step is reported."""
+    dev = _dev()
+    from mouse_core_b200 import kernels as K
+
+    rows = [(50, 3), (300, 330), (0, 40), (700, 1)]
+    args = q, kp, vp, table, cu, kv_len = _paged(rows, 8, 4, hd, 64, seed=room)
+    o, A = _attention_reference(*args, 0.1)
+    T = 3 + room
+    out = torch.full((T + 2, 8, hd), 7.0, dtype=torch.bfloat16, device=dev)
+    K.chunk_attention(q[:T].contiguous(), kp, vp, table, cu, kv_len, 0.1, out=out[:T])
+    assert _status() == 7
+    _check(out[:T], (o[:T], A[:T]))
+    assert bool((out[T:] == 7.0).all())
+    # Fewer cached keys than tokens left out: those that fit see nothing.
+    short = kv_len.clone()
+    short[1] = 5
+    K.chunk_attention(q[:T].contiguous(), kp, vp, table, cu, short, 0.1, out=out[:T])
+    assert _status() == 7
+    _check(out[:3], (o[:3], A[:3]))
+    if room < 325:
+        assert bool((out[3:3 + min(room, 325)] == 0).all())
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_keys_past_the_table_are_left_out_and_reported(hd):
+    _dev()
+    from mouse_core_b200 import kernels as K
+
+    for rows in ([(500, 1), (40, 1)], [(500, 7), (40, 1)], [(400, 200), (70, 30)], [(20, 700), (1, 1)]):
+        q, kp, vp, table, cu, kv_len = _paged(rows, 8, 4, hd, 64, seed=hd)
+        narrow = table[:, :5].contiguous()  # 320 slots
+        out = K.chunk_attention(q, kp, vp, narrow, cu, kv_len, 0.1)
+        assert _status() == 3
+        o, A = _attention_reference(q, kp, vp, table, cu, kv_len, 0.1)
+        # Row 0 again, every token over the table's slots alone.
+        n = rows[0][1]
+        for i in range(n):
+            if rows[0][0] + i >= 320:
+                one = [t.to(q.device) for t in (torch.tensor([0, 1], dtype=torch.int32), torch.tensor([320], dtype=torch.int32))]
+                o[i:i + 1], A[i:i + 1] = _attention_reference(q[i:i + 1], kp, vp, table[:1], *one, 0.1)
+        _check(out, (o, A), rows)
