@@ -370,12 +370,15 @@ class PagedDecodeSession:
         old = self.pages.num_pages
         new = max(2 * old, old + need_free - self.pages.free_pages)
         shape = (self.n_layers, new, self.n_kv_heads, self.page_size, self.head_dim)
+        grown = {}
         for name in ("k_pool", "v_pool"):
             src = getattr(self, name)
-            dst = torch.zeros(shape, device=self.device, dtype=self.dtype)
+            grown[name] = dst = torch.zeros(shape, device=self.device, dtype=self.dtype)
             dst[:, :old] = src
             self._outgrown(src)
-            setattr(self, name, dst)
+            setattr(self, name, dst[:, :old])  # (all there is, should the other one find no memory)
+            del src
+        self.k_pool, self.v_pool = grown["k_pool"], grown["v_pool"]
         self.pages.grow_pool(new)
 
     def _stage(self, n_int32: int) -> torch.Tensor:

@@ -85,6 +85,33 @@ def test_pools_outgrown_on_another_stream_stay_until_that_stream_is_done(recorde
         assert (t.data_ptr(), t.numel(), "side") in recorded
 
 
+def test_a_pool_that_finds_no_memory_to_grow_stays_whole(recorded, monkeypatch):
+    """The second of the two pools cannot be allocated: both keep their pages,
+    layer by layer contiguous, and growing them again works."""
+    s = _stub()
+    s.n_layers, s.n_kv_heads, s.head_dim = 2, 2, 64
+    k, v = (torch.randn(2, 8, 2, 64, 64).bfloat16() for _ in range(2))
+    s.k_pool, s.v_pool = k.clone(), v.clone()
+    real, left = torch.zeros, [1]
+
+    def zeros(*a, **kw):
+        left[0] -= 1
+        if left[0] < 0:
+            raise torch.OutOfMemoryError("zeros")
+        return real(*a, **kw)
+
+    with monkeypatch.context() as m:
+        m.setattr(torch, "zeros", zeros)
+        with pytest.raises(torch.OutOfMemoryError):
+            s._grow_pool(12)
+    assert s.pages.num_pages == s.pages.free_pages == 8
+    assert torch.equal(s.k_pool, k) and torch.equal(s.v_pool, v)
+    assert all(p[li].is_contiguous() for p in (s.k_pool, s.v_pool) for li in range(2))
+    s._grow_pool(12)
+    assert s.k_pool.shape == s.v_pool.shape and s.k_pool.shape[1] == s.pages.num_pages >= 12
+    assert torch.equal(s.k_pool[:, :8], k) and torch.equal(s.v_pool[:, :8], v)
+
+
 def test_metadata_outgrown_on_another_stream_stays_until_that_stream_is_done(recorded, monkeypatch):
     """A padded call that widens the block table and enlarges the metadata buffer."""
     s = _stub()
