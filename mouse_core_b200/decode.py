@@ -681,13 +681,13 @@ class PagedDecodeSession:
                 return (x, tuple(x for _ in range(self.n_layers))) if output_hidden_states else x
             try:
                 out = self._body(x, q_pos, kv_len, slot, 0, output_hidden_states, cu_q)
+                if output_hidden_states:
+                    h, hiddens = out
+                    return self._final(h), tuple(t.to(self.dtype) for t in hiddens)
+                return self._final(out)
             except BaseException:
                 self._len = before  # (slots behind a row's length are never read)
                 raise
-            if output_hidden_states:
-                h, hiddens = out
-                return self._final(h), tuple(t.to(self.dtype) for t in hiddens)
-            return self._final(out)
 
     def _final(self, h: torch.Tensor, copy: bool = False) -> torch.Tensor:
         """The model's final norm, in the model's dtype (a fresh tensor when

@@ -396,6 +396,14 @@ def test_a_packed_call_that_raised_can_be_made_again(monkeypatch):
     run([1, 130, 2], "chunk_attention")
     run([1, 1, 300], "chunk_plan")
     run([5, 0, 1])
+    run([1, 2, 1])
+    lengths, x = sess.lengths.tolist(), torch.randn(3, D, device=dev).bfloat16()
+    with monkeypatch.context() as m:
+        m.setattr(sess, "_final", lambda h: 1 / 0)
+        with pytest.raises(ZeroDivisionError):
+            sess.forward_packed(embeds=x, lengths=[1, 0, 2])
+    assert sess.lengths.tolist() == lengths
+    run([1, 0, 2])
     from mouse_core_b200 import _lib
 
     assert _lib.device_status() == 0
