@@ -14,7 +14,7 @@
 // sub-tiles of TS = 128 / G tokens (128 query rows) each. (A big tile with one
 // sub-tile's tokens takes its even key tiles as the one and its odd ones as the
 // other, "dual", and the epilogue joins the two: 3 rows of up to 20 query rows over
-// 131000 keys take 147 us, and 167 without.) Every (tile,
+// 131000 keys take 141 us, and 154 without.) Every (tile,
 // kv-head) is one item over 128-key tiles of the cache; items with many key
 // tiles are split along the keys into pieces when the step has too few items
 // to fill the SMs (chunk_plan_kernel): each piece leaves (O, max, sum) in fp32,
@@ -45,13 +45,19 @@
 // 3650, and a piece costs 3000 more to start and to end.
 // Measured, with the plan (16/8 heads of 128 in 128-token pages, or 32/8 of 64 in
 // 64-token pages; 6.55 TB/s copied and 1677 TFLOP/s multiplied by the library):
-//   256 single tokens over 64..4096 keys           350 us, 6.2 TB/s
-//   128 rows of 0..4 tokens over 128..16380 (64)   119 us, 5.8 TB/s
+//   256 single tokens over 64..4096 keys           366 us, 6.0 TB/s
+//   128 rows of 0..4 tokens over 128..16380 (64)   124 us, 5.6 TB/s
 //   48 rows, four of them windows of 1024           72 us
-//   48 x 256 tokens over 1024..8192 keys           535 us, 890 TFLOP/s
-//   64 windows of 500..1024 from empty (64)        401 us, 395 TFLOP/s
-//   700 tokens over 60001 keys                     420 us, 820 TFLOP/s
-//   3 rows of 1..5 tokens over 90000..131000 (64)  142 us, 4.8 TB/s
+//   48 x 256 tokens over 1024..8192 keys           543 us, 878 TFLOP/s
+//   64 windows of 500..1024 from empty (64)        402 us, 394 TFLOP/s
+//   700 tokens over 60001 keys                     428 us, 810 TFLOP/s
+//   3 rows of 1..5 tokens over 90000..131000 (64)  144 us, 4.7 TB/s
+//
+// Precision: scores, statistics, sums, O and the partials are fp32. The weights
+// are rounded to bf16 for P V, whose V is bf16 (a wider P would need the tf32
+// pipe at half the rate and V converted), and the output once: against 64 bits
+// the outputs are off by 0.0020 to 0.0023 (relative, in the mean square), by
+// 0.0016 to 0.0017 with the output's rounding alone.
 //
 // Every wait is bounded (common.cuh); the first one that runs out stops its
 // CTA. A query row's output (or partial) is written only when the row is done,
